@@ -314,6 +314,51 @@ int rwkv_moe_expert_mix_rows(const void* x, const void* prev, const void* x_k,
 int rwkv_grouped_gemm(const void* a, const void* w, const int32_t* offs, void* out, int M, int N, int K,
                       int G, long long ldo, int epi, int dtype, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Routing to experts from logits (no counterpart in the reference, whose router is
+ * rwkv_moe_router; this is the form with sigmoid or softmax scores, a balance bias and
+ * groups).  logits (n, E) in dtype, row pitch ld elements; E <= 512, k <= 32.
+ *   s = sigmoid(l) (sigmoid != 0) or softmax(l), in fp32;  key = s + bias (bias (E,)
+ *   fp32 or NULL; softmax without a bias compares l itself).  The E experts are
+ *   `groups` (<= 32) equal runs; a run's score is its largest key or, with group_top2,
+ *   the sum of its two largest; the `keep` best runs stay and the k largest keys in them
+ *   are chosen, in descending order.  Ties go to the lower index; NaN ranks first.
+ *   inds (n, k) int32; weights (n, k) fp32 = scale * s / sum of the selected s
+ *   (renormalize; 0 where that sum is 0) or scale * s; counts int32[E] or NULL: rows
+ *   given to each expert.  n = 0 is valid.
+ * rwkv_route_experts_backward: dlogits (n, E) contiguous in dtype from dweights (n, k)
+ *   fp32 and the forward's inds and weights (same k, sigmoid, renormalize, scale).  The
+ *   selection is constant; the bias has no gradient. */
+int rwkv_route_experts(const void* logits, long long ld, const float* bias, int32_t* inds, float* weights,
+                       int32_t* counts, int n, int E, int k, int groups, int keep, int group_top2, int sigmoid,
+                       int renormalize, float scale, int dtype, void* stream);
+int rwkv_route_experts_backward(const void* logits, long long ld, const int32_t* inds, const float* weights,
+                                const float* dweights, void* dlogits, int n, int E, int k, int sigmoid,
+                                int renormalize, float scale, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Products in 8-bit floating point (e4m3), no counterpart in the reference.
+ * A block of 128 values with a = max(max|x|, 1e-30) stands as q = e4m3(x * (448 / a)) with
+ * the fp32 scale a / 448.
+ * rwkv_quantize_fp8_rows: x (M, K) in dtype, row pitch ldx -> q (M, K) bytes, row pitch
+ *   ldq (8-byte aligned), scale (ceil(K / 128), M): one scale per row and 128 columns.
+ * rwkv_quantize_fp8_weight: w (G, N, K) contiguous in dtype -> q (G * N rows, pitch ldq,
+ *   16-byte aligned), scale (G, ceil(N / 128), ceil(K / 128)): one per 128 x 128 block.
+ * rwkv_fp8_gemm: for the rows m in [offs[g], offs[g + 1]) of group g
+ *   out[m, n] = epi( sum_kb a_scale[kb, m] w_scale[g, n / 128, kb] sum_{k in kb} a[m, k] w[g, n, k] )
+ *   with fp32 sums; a (M, K) pitch lda, w (G, N, K) pitch ldw and group pitch
+ *   w_group_stride, all in bytes and multiples of 16 on 16-byte aligned bases; G <= 256;
+ *   offs (G + 1) ascending int32 on the device, or NULL with G = 1.  out (M, N), row
+ *   pitch ldo elements, in out_dtype; epi 0: the product, epi 1: relu(.)^2 of it.  Rows
+ *   outside every group are not written.  M = 0 is valid. */
+int rwkv_quantize_fp8_rows(const void* x, long long ldx, void* q, long long ldq, float* scale, int M, int K,
+                           int dtype, void* stream);
+int rwkv_quantize_fp8_weight(const void* w, void* q, long long ldq, float* scale, int G, int N, int K, int dtype,
+                             void* stream);
+int rwkv_fp8_gemm(const void* a, long long lda, const float* a_scale, const void* w, long long ldw,
+                  long long w_group_stride, const float* w_scale, const int32_t* offs, void* out, long long ldo,
+                  int M, int N, int K, int G, int epi, int out_dtype, void* stream);
+
 /* sum_{i<j} ||A_i^T A_j||_F^2 over the expert down-projections
  * (LoRAMoE_CMix.orthogonal_loss, moe.py:149-163).  A (E, C, R) dtype;
  * out: one fp32 scalar.  R <= 64.                                          */

@@ -6,6 +6,7 @@ present, the public functions raise instead of falling back to anything else.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -30,6 +31,8 @@ DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
+_LL = ctypes.c_longlong
+_F = ctypes.c_float
 
 # name -> (restype, argtypes); must match include/rwkv_b200.h
 SIGNATURES = {
@@ -67,6 +70,11 @@ SIGNATURES = {
     "rwkv_moe_lora_up": (_I, [_P] * 5 + [_I] * 5 + [_P]),
     "rwkv_moe_combine_rows": (_I, [_P] * 5 + [_I] * 4 + [_P]),
     "rwkv_moe_expert_mix_rows": (_I, [_P] * 6 + [_I] * 6 + [_P]),
+    "rwkv_route_experts": (_I, [_P, _LL] + [_P] * 4 + [_I] * 8 + [_F, _I, _P]),
+    "rwkv_route_experts_backward": (_I, [_P, _LL] + [_P] * 4 + [_I] * 5 + [_F, _I, _P]),
+    "rwkv_quantize_fp8_rows": (_I, [_P, _LL, _P, _LL, _P, _I, _I, _I, _P]),
+    "rwkv_quantize_fp8_weight": (_I, [_P, _P, _LL, _P] + [_I] * 4 + [_P]),
+    "rwkv_fp8_gemm": (_I, [_P, _LL, _P, _P, _LL, _LL, _P, _P, _P, _LL] + [_I] * 6 + [_P]),
     "rwkv_grouped_gemm": (_I, [_P] * 4 + [_I] * 4 + [ctypes.c_longlong, _I, _I, _P]),
     "rwkv_head_ce_workspace_size": (_SZ, [_I, _I]),
     "rwkv_head_ce_stats": (_I, [_P] * 4 + [_I] * 3 + [_P, _SZ, _I, _P]),
@@ -87,6 +95,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_HERE = contextlib.nullcontext()
 
 
 class RwkvNativeError(RuntimeError):
@@ -132,6 +141,8 @@ KERNELS_PER_CALL = {
     "rwkv_moe_lora_up": 1, "rwkv_moe_combine_rows": 1, "rwkv_lerp": 1, "rwkv_lerp_prev": 1, "rwkv_lerp_prev_state": 1, "rwkv_tmix_mid": 1,
     "rwkv_tmix_post": 1, "rwkv_relu_sq": 1, "rwkv_lora_act": 1, "rwkv_argmax_rows": 1, "rwkv_add_layernorm": 1, "rwkv_moe_expert_mix_rows": 1,
     "rwkv_ce_chunk": 1, "rwkv_ce_finalize": 1, "rwkv_ce_chunk_grad": 1,
+    "rwkv_route_experts": 1, "rwkv_route_experts_backward": 1, "rwkv_quantize_fp8_rows": 1, "rwkv_quantize_fp8_weight": 1,
+    "rwkv_fp8_gemm": 1,
     "rwkv_grouped_gemm": 1, "rwkv_head_ce_stats": 2, "rwkv_head_ce_grad": 1,
 }
 launch_count = 0
@@ -154,6 +165,25 @@ def ptr(t: torch.Tensor | None):
 
 def stream_ptr(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def on_device(dev: torch.device):
+    """``torch.cuda.device(dev)``, or nothing to enter when ``dev`` is current already."""
+    if dev.type != "cuda":
+        raise ValueError(f"the tensors must be on a CUDA device, not {dev}")
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def rows_2d(t: torch.Tensor) -> torch.Tensor:
+    """``t`` (..., C) as (rows, C) with unit column stride, copied only where no view has that."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def row_stride(t: torch.Tensor) -> int:
+    """Row pitch of a 2-d tensor in elements (any multiple of 16 does for a single row)."""
+    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 16) * 16
 
 
 def dtype_code(t: torch.Tensor) -> int:

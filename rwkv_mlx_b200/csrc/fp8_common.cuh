@@ -1,0 +1,46 @@
+// Shared by the e4m3 kernels: the scale of a block and the conversions.
+//
+// A block of 128 values with a = max|x| (at least FP8_TINY) stands as q_i = e4m3(x_i * (448 / a))
+// with the scale a / 448.  448 / a is formed as reciprocal(a) * 448 and a / 448 as
+// a * (1 / 448), each operation rounded once in fp32.  FP8_TINY keeps 448 / a finite; values below
+// it lose bits, an all-zero block keeps the scale FP8_TINY / 448.  A NaN stays a NaN in its own
+// place (fmaxf passes over it); an infinity makes its block's scale infinite and itself NaN.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace rwkv {
+namespace fp8 {
+constexpr int BLK = 128;
+constexpr float E4M3_MAX = 448.f, FP8_TINY = 1e-30f;
+
+__device__ __forceinline__ float clamp_amax(float a) { return fmaxf(a, FP8_TINY); }
+__device__ __forceinline__ float quant_mul(float a) { return __fmul_rn(__frcp_rn(a), E4M3_MAX); }
+__device__ __forceinline__ float dequant_scale(float a) { return __fmul_rn(a, 1.f / E4M3_MAX); }
+
+// Two floats to two e4m3 bytes (lower address: lo), round to nearest even.
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+    return pack2(a, b) | (pack2(c, d) << 16);
+}
+
+// 8 consecutive values as floats (16-byte aligned).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&o)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 x0 = *reinterpret_cast<const float4*>(p), x1 = *reinterpret_cast<const float4*>(p + 4);
+        o[0] = x0.x, o[1] = x0.y, o[2] = x0.z, o[3] = x0.w, o[4] = x1.x, o[5] = x1.y, o[6] = x1.z, o[7] = x1.w;
+    } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        const T* h = reinterpret_cast<const T*>(&x);
+#pragma unroll
+        for (int q = 0; q < 8; q++) o[q] = to_f32(h[q]);
+    }
+}
+}  // namespace fp8
+}  // namespace rwkv

@@ -1,0 +1,29 @@
+// Arguments of the e4m3 products (fp8_gemm.cu: few rows, fp8_gemm_tc.cu: tcgen05).
+#pragma once
+#include "fp8_common.cuh"
+
+namespace rwkv {
+namespace fp8 {
+
+enum Epi { STORE = 0, RELU2 = 1, RELU2_Q = 2 };
+
+struct GemmArgs {
+    const uint8_t* a;   // (M, K), row pitch lda
+    long long lda;
+    const float* as;    // (ceil(K / 128), M)
+    const uint8_t* w;   // (G, N, K), row pitch ldw, group pitch gsw
+    long long ldw, gsw;
+    const float* ws;    // (G, ceil(N / 128), ceil(K / 128))
+    const int32_t* offs;
+    void* out;          // (M, N), row pitch ldo (elements of the output type)
+    long long ldo;
+    float* os;          // RELU2_Q: (ceil(N / 128), M) scales of the output rows
+    int M, N, K, G;
+};
+
+int gemm_stream(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st);
+int gemm_tc(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st);
+bool gemm_prefers_stream(int M, int N, int K, int G);
+
+}  // namespace fp8
+}  // namespace rwkv

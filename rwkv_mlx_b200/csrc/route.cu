@@ -1,0 +1,382 @@
+// Routing to experts from logits (n, E): scores, balance bias, groups, top-k, weights, and
+// the gradient of the logits.
+//
+//   s_e   = sigmoid(l_e)  or  softmax(l)_e
+//   key_e = s_e + bias_e  (softmax without a bias: l_e itself, which has the same order and
+//           no rounding of its own)
+//   a group's score is its largest key or the sum of its two largest; the `keep` best groups
+//   stay, and the k largest keys among them are chosen.  Ties go to the lower index, NaN keys
+//   rank above all others (so a NaN logit reaches the weights instead of vanishing), and a
+//   row of -inf still yields k distinct experts, with weights 0.
+//   w_j   = scale * s_j / sum_selected s   or   scale * s_j
+//
+// One warp per token.  Lane i holds the EPL consecutive experts from i * EPL on, so the
+// lowest lane of a tie also has the lowest expert, and a group is a run of lanes when EPL
+// divides its size.  Keys are compared as unsigned integers that order like the floats: a
+// round of the top-k is one redux.sync over the lanes' best keys, a ballot and a rescan of
+// the winner's EPL keys.  expf and the reciprocal are CUDA's correctly rounded or
+// few-ulp functions, not the fast forms, so that keys agree with the formula evaluated in
+// fp32 elsewhere and no near-tie flips.
+#include "common.cuh"
+
+namespace rwkv {
+namespace route {
+
+constexpr int NT = 256, NW = NT / 32, MAXE = 512, MAXK = 32, MAXG = 32;
+
+struct Args {
+    const void* logits;
+    long long ld;
+    const float* bias;
+    int32_t* inds;
+    float* weights;
+    int32_t* counts;
+    int n, E, k, groups, keep, top2, renorm, sigmoid;
+    int vec;  // rows 16-byte aligned
+    float scale;
+};
+
+// Unsigned order of a float: NaN highest, -0 equal to +0.  Never 0 (the excluded key).
+__device__ __forceinline__ uint32_t okey(float f) {
+    if (f != f) return 0xffffffffu;
+    const uint32_t u = __float_as_uint(f + 0.f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float sigmoidf(float x) { return __frcp_rn(1.f + expf(-x)); }
+
+__device__ __forceinline__ float wmax(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const float t = __shfl_xor_sync(0xffffffffu, v, o);
+        v = (t > v || t != t) ? t : v;  // NaN wins
+    }
+    return v;
+}
+__device__ __forceinline__ float wsum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// The lane's EPL logits of a row (experts past E: -inf).
+template <typename T, int EPL>
+__device__ __forceinline__ void load_row(const T* row, int e0, int E, bool vec, float (&l)[EPL]) {
+    constexpr int BYTES = EPL * sizeof(T), V = BYTES >= 16 ? 16 : BYTES, PER = V / sizeof(T);
+    if (vec && e0 + EPL <= E) {
+#pragma unroll
+        for (int i = 0; i < EPL; i += PER) {
+            alignas(16) T t[PER];
+            if constexpr (V == 16) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(row + e0 + i);
+            else if constexpr (V == 8) *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(row + e0 + i);
+            else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(t) = *reinterpret_cast<const uint32_t*>(row + e0 + i);
+            else t[0] = row[e0 + i];
+#pragma unroll
+            for (int q = 0; q < PER; q++) l[i + q] = to_f32(t[q]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < EPL; i++) l[i] = e0 + i < E ? to_f32(row[e0 + i]) : -INFINITY;
+    }
+}
+
+// Two largest of (a1 >= a2) and (b1 >= b2) as ordered keys.
+__device__ __forceinline__ void merge2(uint32_t& a1, uint32_t& a2, uint32_t b1, uint32_t b2) {
+    const uint32_t lo = min(a1, b1);
+    a1 = max(a1, b1);
+    a2 = max(lo, max(a2, b2));
+}
+__device__ __forceinline__ float unkey(uint32_t u) {
+    if (u == 0xffffffffu) return __int_as_float(0x7fc00000);
+    return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+
+template <typename T, int EPL>
+__global__ void __launch_bounds__(NT) route_kernel(const Args p) {
+    extern __shared__ uint32_t smem_route[];
+    uint32_t* hist = smem_route;                                        // E counters (counts only)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E;
+    uint32_t* wkeys = smem_route + (p.counts ? E : 0) + warp * E;       // this warp's keys (odd group sizes only)
+    if (p.counts) {
+        for (int e = threadIdx.x; e < E; e += NT) hist[e] = 0;
+        __syncthreads();
+    }
+    const int e0 = lane * EPL, per = E / p.groups;
+    const int lanes_per = per / EPL;  // lanes of a group, when the layout is aligned
+    const bool by_lanes = per % EPL == 0 && (lanes_per & (lanes_per - 1)) == 0;
+    float b[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; i++) b[i] = p.bias && e0 + i < E ? p.bias[e0 + i] : 0.f;
+
+    for (int t = blockIdx.x * NW + warp; t < p.n; t += gridDim.x * NW) {
+        const T* row = reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld;
+        float l[EPL];
+        load_row<T, EPL>(row, e0, E, p.vec, l);
+        float m = 0.f, z = 0.f;  // softmax: row maximum (0 for a row of -inf) and sum
+        const bool by_logit = !p.sigmoid && !p.bias && !(p.groups > 1 && p.top2);
+        if (!p.sigmoid && (!by_logit || !p.renorm)) {
+            m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < EPL; i++) m = (l[i] > m || l[i] != l[i]) ? l[i] : m;
+            m = wmax(m);
+            if (m == -INFINITY) m = 0.f;
+#pragma unroll
+            for (int i = 0; i < EPL; i++) z += expf(l[i] - m);
+            z = wsum(z);
+        }
+        uint32_t key[EPL];
+#pragma unroll
+        for (int i = 0; i < EPL; i++) {
+            float f = l[i];
+            if (p.sigmoid) f = sigmoidf(f);
+            else if (!by_logit) f = z == 0.f ? 0.f : expf(f - m) / z;
+            if (p.bias) f += b[i];
+            key[i] = e0 + i < E ? okey(f) : 0u;
+        }
+        if (p.groups > 1) {
+            uint32_t g1 = 0, g2 = 0;  // two largest keys of this lane's group
+            int mine;                 // the group that this lane ranks
+            if (by_lanes) {
+#pragma unroll
+                for (int i = 0; i < EPL; i++) merge2(g1, g2, key[i], 0u);
+                for (int o = 1; o < lanes_per; o <<= 1)
+                    merge2(g1, g2, __shfl_xor_sync(0xffffffffu, g1, o), __shfl_xor_sync(0xffffffffu, g2, o));
+                mine = lane / lanes_per;
+            } else {
+#pragma unroll
+                for (int i = 0; i < EPL; i++)
+                    if (e0 + i < E) wkeys[e0 + i] = key[i];
+                __syncwarp();
+                mine = lane;
+                if (lane < p.groups)
+                    for (int i = 0; i < per; i++) merge2(g1, g2, wkeys[lane * per + i], 0u);
+                __syncwarp();
+            }
+            uint32_t gs = g1;
+            if (p.top2 && per > 1) gs = okey(unkey(g1) + unkey(g2));
+            int rank = 0;
+            for (int g = 0; g < p.groups; g++) {
+                const uint32_t o = __shfl_sync(0xffffffffu, gs, by_lanes ? g * lanes_per : g);
+                rank += (o > gs || (o == gs && g < mine)) ? 1 : 0;
+            }
+            const uint32_t stay = __ballot_sync(0xffffffffu, rank < p.keep && mine < p.groups);
+            if (by_lanes) {
+                if (!((stay >> lane) & 1u)) {
+#pragma unroll
+                    for (int i = 0; i < EPL; i++) key[i] = 0u;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < EPL; i++)
+                    if (e0 + i < E && !((stay >> ((e0 + i) / per)) & 1u)) key[i] = 0u;
+            }
+        }
+        // top-k: lane j ends up with the j-th choice
+        uint32_t best = 0;
+        int bi = 0, choice = 0;
+#pragma unroll
+        for (int i = 0; i < EPL; i++)
+            if (key[i] > best) best = key[i], bi = i;
+        for (int j = 0; j < p.k; j++) {
+            const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+            const int src = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+            const int e = __shfl_sync(0xffffffffu, e0 + bi, src);
+            if (lane == j) choice = e;
+            if (lane == src) {
+                best = 0;
+                const int gone = bi;
+#pragma unroll
+                for (int i = 0; i < EPL; i++) {
+                    if (i == gone) key[i] = 0u;
+                    if (key[i] > best) best = key[i], bi = i;
+                }
+            }
+        }
+        const bool on = lane < p.k;
+        float s = 0.f;
+        if (p.sigmoid) {
+            if (on) s = sigmoidf(to_f32(row[choice]));
+        } else {
+            const float lj = on ? to_f32(row[choice]) : -INFINITY;
+            if (p.renorm) {  // the row's sum cancels: exponentials relative to the largest selected logit
+                m = wmax(lj);
+                if (m == -INFINITY) m = 0.f;
+                s = on ? expf(lj - m) : 0.f;
+            } else if (on) {
+                s = z == 0.f ? 0.f : expf(lj - m) / z;
+            }
+        }
+        if (p.renorm) {
+            const float sum = wsum(s);
+            s = sum == 0.f ? 0.f : s / sum;
+        }
+        if (on) {
+            p.inds[(long long)t * p.k + lane] = choice;
+            p.weights[(long long)t * p.k + lane] = s * p.scale;
+            if (p.counts) atomicAdd(&hist[choice], 1u);
+        }
+    }
+    if (p.counts) {
+        __syncthreads();
+        for (int e = threadIdx.x; e < E; e += NT) {
+            if (gridDim.x == 1) p.counts[e] = (int)hist[e];
+            else if (hist[e]) atomicAdd(&p.counts[e], (int)hist[e]);  // integers: any order gives the same sum
+        }
+    }
+}
+
+struct BwdArgs {
+    const void* logits;
+    long long ld;
+    const int32_t* inds;
+    const float* weights;
+    const float* dw;
+    void* dlogits;  // (n, E) contiguous
+    int n, E, k, renorm, sigmoid, vec;
+    float scale;
+};
+
+// d loss / d logits.  With w the forward's weights, wn = w / scale:
+//   renormalised: t_j = w_j (g_j - sum_i g_i wn_i);  softmax dl_j = t_j, sigmoid dl_j = t_j (1 - s_j);
+//   sigmoid, not renormalised: dl_j = g_j w_j (1 - s_j);
+//   these are zero off the selection, and only softmax without renormalising is dense:
+//   dl_e = s_e (scale g_e [e selected] - sum_i g_i w_i).
+template <typename T, int EPL>
+__global__ void __launch_bounds__(NT) route_bwd_kernel(const BwdArgs p) {
+    extern __shared__ float smem_route_bwd[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E, e0 = lane * EPL;
+    float* d = smem_route_bwd + warp * (32 * EPL);  // the row's sparse part, zero between tokens
+#pragma unroll
+    for (int i = 0; i < EPL; i++) d[e0 + i] = 0.f;
+    __syncwarp();
+    const bool dense = !p.sigmoid && !p.renorm;
+    for (int t = blockIdx.x * NW + warp; t < p.n; t += gridDim.x * NW) {
+        const T* row = reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld;
+        const bool on = lane < p.k;
+        const int e = on ? p.inds[(long long)t * p.k + lane] : 0;
+        const float w = on ? p.weights[(long long)t * p.k + lane] : 0.f;
+        const float g = on ? p.dw[(long long)t * p.k + lane] : 0.f;
+        const bool fine = on && (unsigned)e < (unsigned)E;
+        float v = 0.f, dot = 0.f;
+        if (p.renorm || dense) dot = wsum(g * w);
+        if (p.renorm) v = w * (g - (p.scale == 0.f ? 0.f : dot / p.scale));
+        else if (p.sigmoid) v = g * w;
+        else v = g * p.scale;
+        if (p.sigmoid && fine) v *= sigmoidf(-to_f32(row[e]));
+        if (fine) d[e] = v;
+        __syncwarp();
+        float o[EPL];
+#pragma unroll
+        for (int i = 0; i < EPL; i++) o[i] = d[e0 + i];
+        __syncwarp();
+        if (fine) d[e] = 0.f;
+        __syncwarp();
+        if (dense) {
+            float l[EPL], m = -INFINITY, z = 0.f;
+            load_row<T, EPL>(row, e0, E, p.vec, l);
+#pragma unroll
+            for (int i = 0; i < EPL; i++) m = (l[i] > m || l[i] != l[i]) ? l[i] : m;
+            m = wmax(m);
+            if (m == -INFINITY) m = 0.f;
+#pragma unroll
+            for (int i = 0; i < EPL; i++) l[i] = expf(l[i] - m), z += l[i];
+            z = wsum(z);
+            const float inv = z == 0.f ? 0.f : 1.f / z;
+#pragma unroll
+            for (int i = 0; i < EPL; i++) o[i] = l[i] * inv * (o[i] - dot);
+        }
+        T* out = reinterpret_cast<T*>(p.dlogits) + (long long)t * E;
+        constexpr int BYTES = EPL * sizeof(T), V = BYTES >= 16 ? 16 : BYTES, PER = V / sizeof(T);
+        if (p.vec && e0 + EPL <= E) {
+#pragma unroll
+            for (int i = 0; i < EPL; i += PER) {
+                alignas(16) T r[PER];
+#pragma unroll
+                for (int q = 0; q < PER; q++) r[q] = from_f32<T>(o[i + q]);
+                if constexpr (V == 16) *reinterpret_cast<uint4*>(out + e0 + i) = *reinterpret_cast<uint4*>(r);
+                else if constexpr (V == 8) *reinterpret_cast<uint2*>(out + e0 + i) = *reinterpret_cast<uint2*>(r);
+                else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(out + e0 + i) = *reinterpret_cast<uint32_t*>(r);
+                else out[e0 + i] = r[0];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < EPL; i++)
+                if (e0 + i < E) out[e0 + i] = from_f32<T>(o[i]);
+        }
+    }
+}
+
+static int grid_for(int n, int per_sm) {
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const long long want = ((long long)n + NW - 1) / NW;
+    return (int)(want < (long long)sms * per_sm ? want : (long long)sms * per_sm);
+}
+
+template <typename T, int EPL>
+static void launch_fwd(const Args& p, int grid, cudaStream_t st) {
+    const int per = p.E / p.groups, lp = per / EPL;
+    const bool by_lanes = per % EPL == 0 && (lp & (lp - 1)) == 0;
+    const size_t smem = sizeof(uint32_t) * ((p.counts ? p.E : 0) + (p.groups > 1 && !by_lanes ? NW * p.E : 0));
+    route_kernel<T, EPL><<<grid, NT, smem, st>>>(p);
+}
+template <typename T, int EPL>
+static void launch_bwd(const BwdArgs& p, int grid, cudaStream_t st) {
+    route_bwd_kernel<T, EPL><<<grid, NT, sizeof(float) * NW * 32 * EPL, st>>>(p);
+}
+
+}  // namespace route
+}  // namespace rwkv
+
+using namespace rwkv;
+
+// EPL: the smallest power of two that covers E with 32 lanes.
+#define ROUTE_BY_E(E, CALL)       \
+    if ((E) <= 32) { CALL(1) }    \
+    else if ((E) <= 64) { CALL(2) } \
+    else if ((E) <= 128) { CALL(4) } \
+    else if ((E) <= 256) { CALL(8) } \
+    else { CALL(16) }
+
+extern "C" int rwkv_route_experts(const void* logits, long long ld, const float* bias, int32_t* inds, float* weights,
+                                  int32_t* counts, int n, int E, int k, int groups, int keep, int group_top2,
+                                  int sigmoid, int renormalize, float scale, int dtype, void* stream) {
+    if (dtype != RWKV_F32 && dtype != RWKV_F16 && dtype != RWKV_BF16) return RWKV_ERR_DTYPE;
+    if (n < 0 || E <= 0 || E > route::MAXE || k <= 0 || k > route::MAXK || ld < E) return RWKV_ERR_SHAPE;
+    if (groups <= 0 || groups > route::MAXG || E % groups || keep <= 0 || keep > groups) return RWKV_ERR_SHAPE;
+    if (k > keep * (E / groups)) return RWKV_ERR_SHAPE;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (n == 0) return counts ? set_cuda_error(cudaMemsetAsync(counts, 0, sizeof(int32_t) * E, st)) : RWKV_OK;
+    if (!logits || !inds || !weights) return RWKV_ERR_ARG;
+    const int es = dtype == RWKV_F32 ? 4 : 2;
+    route::Args p{logits, ld, bias, inds, weights, counts, n, E, k, groups, keep, group_top2, renormalize, sigmoid, 0, scale};
+    p.vec = aligned(logits, 16) && (ld * es) % 16 == 0;
+    const int grid = route::grid_for(n, 8);
+    if (counts && grid > 1) {
+        const int rc = set_cuda_error(cudaMemsetAsync(counts, 0, sizeof(int32_t) * E, st));
+        if (rc) return rc;
+    }
+    RWKV_DISPATCH_DTYPE(dtype, T, {
+#define ROUTE_FWD(EPL) route::launch_fwd<T, EPL>(p, grid, st);
+        ROUTE_BY_E(E, ROUTE_FWD)
+    });
+    return check_launch();
+}
+
+extern "C" int rwkv_route_experts_backward(const void* logits, long long ld, const int32_t* inds, const float* weights,
+                                           const float* dweights, void* dlogits, int n, int E, int k, int sigmoid,
+                                           int renormalize, float scale, int dtype, void* stream) {
+    if (dtype != RWKV_F32 && dtype != RWKV_F16 && dtype != RWKV_BF16) return RWKV_ERR_DTYPE;
+    if (n < 0 || E <= 0 || E > route::MAXE || k <= 0 || k > route::MAXK || k > E || ld < E) return RWKV_ERR_SHAPE;
+    if (n == 0) return RWKV_OK;
+    if (!logits || !inds || !weights || !dweights || !dlogits) return RWKV_ERR_ARG;
+    const int es = dtype == RWKV_F32 ? 4 : 2;
+    route::BwdArgs p{logits, ld, inds, weights, dweights, dlogits, n, E, k, renormalize, sigmoid, 0, scale};
+    p.vec = aligned(logits, 16) && (ld * es) % 16 == 0 && aligned(dlogits, 16) && ((long long)E * es) % 16 == 0;
+    const int grid = route::grid_for(n, 8);
+    cudaStream_t st = (cudaStream_t)stream;
+    RWKV_DISPATCH_DTYPE(dtype, T, {
+#define ROUTE_BWD(EPL) route::launch_bwd<T, EPL>(p, grid, st);
+        ROUTE_BY_E(E, ROUTE_BWD)
+    });
+    return check_launch();
+}

@@ -1,0 +1,202 @@
+"""Products in 8-bit floating point (e4m3) with an fp32 scale for each block of 128.
+
+Activations carry one scale for each 128 values of a row, weights one for each 128 x 128 block
+(``csrc/fp8_quant.cu``); products accumulate in fp32 and apply the scales block by block
+(``csrc/fp8_gemm.cu``, ``csrc/fp8_gemm_tc.cu``).  The reference has no 8-bit path; these are the
+weights-in-8-bits forms of the projections of rwkv_mlx/model.py:245-263 and of the experts of
+rwkv_mlx/moe.py:231-239.
+
+Layouts: an e4m3 matrix is ``torch.float8_e4m3fn`` with unit column stride, its rows 16-byte aligned
+(the quantisers here pad the row pitch for that); row scales are (M, ceil(K / 128)) fp32 stored with
+the rows contiguous, weight scales (..., ceil(N / 128), ceil(K / 128)) fp32 contiguous.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native as nat
+
+BLOCK = 128
+E4M3 = torch.float8_e4m3fn
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _empty_e4m3(rows: int, cols: int, dev) -> torch.Tensor:
+    pitch = -(-cols // 16) * 16
+    t = torch.empty((rows, pitch), device=dev, dtype=E4M3)
+    return t if pitch == cols else t[:, :cols]
+
+
+def quantize_fp8_rows(x: torch.Tensor):
+    """x (M, K) fp32 / fp16 / bf16 -> (q (M, K) e4m3, scale (M, ceil(K / 128)) fp32).
+
+    For each block of 128 values of a row, a = max|x| (at least 1e-30): scale = a / 448,
+    q = e4m3(x * (448 / a)).  A NaN stays NaN in its place; an infinity makes its block NaN."""
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError("quantize_fp8_rows: x must be (M, K) with K >= 1")
+    code = nat.dtype_code(x)
+    x = nat.rows_2d(x)
+    M, K = x.shape
+    dev = x.device
+    q = _empty_e4m3(M, K, dev)
+    scale = torch.empty((_blocks(K), M), device=dev, dtype=torch.float32)
+    L = nat.lib()
+    with nat.on_device(dev):
+        rc = L.rwkv_quantize_fp8_rows(nat.ptr(x), nat.row_stride(x), nat.ptr(q), q.stride(0), nat.ptr(scale), M, K, code,
+                                      nat.stream_ptr(dev))
+    nat.check(rc, "rwkv_quantize_fp8_rows")
+    return q, scale.t()
+
+
+def quantize_fp8_weight(w: torch.Tensor):
+    """w (N, K) or (G, N, K) -> (q e4m3 of the same shape, scale (.., ceil(N / 128), ceil(K / 128)))."""
+    if w.dim() not in (2, 3) or min(w.shape) < 1:
+        raise ValueError("quantize_fp8_weight: w must be (N, K) or (G, N, K), not empty")
+    code = nat.dtype_code(w)
+    w = w.detach().contiguous()
+    G, (N, K) = (1 if w.dim() == 2 else w.shape[0]), w.shape[-2:]
+    dev = w.device
+    q = _empty_e4m3(G * N, K, dev)
+    scale = torch.empty((G, _blocks(N), _blocks(K)), device=dev, dtype=torch.float32)
+    L = nat.lib()
+    with nat.on_device(dev):
+        rc = L.rwkv_quantize_fp8_weight(nat.ptr(w), nat.ptr(q), q.stride(0), nat.ptr(scale), G, N, K, code,
+                                        nat.stream_ptr(dev))
+    nat.check(rc, "rwkv_quantize_fp8_weight")
+    if w.dim() == 2:
+        return q, scale[0]
+    return q.unflatten(0, (G, N)), scale
+
+
+def transpose_fp8_weight(q: torch.Tensor, scale: torch.Tensor):
+    """The same weight laid out (.., K, N), for products with its transpose (the gradient of the
+    input): bytes and scales move, no value changes."""
+    K, N = q.shape[-1], q.shape[-2]
+    lead = q.shape[:-2]
+    rows = K
+    for d in lead:
+        rows *= d
+    out = _empty_e4m3(rows, N, q.device)
+    out = out.unflatten(0, (*lead, K)) if lead else out
+    out.view(torch.uint8).copy_(q.view(torch.uint8).transpose(-1, -2))
+    return out, scale.transpose(-1, -2).contiguous()
+
+
+def _check_rows(name, a, a_scale):
+    if a.dim() != 2 or a.dtype != E4M3 or a.shape[1] < 1:
+        raise ValueError(f"{name}: the rows must be an e4m3 matrix (M, K)")
+    M, K = a.shape
+    if a_scale.shape != (M, _blocks(K)) or a_scale.dtype != torch.float32 or a_scale.device != a.device:
+        raise ValueError(f"{name}: the rows' scales must be fp32 (M, ceil(K / 128)) on the rows' device")
+    if M > 0 and (a.stride(1) != 1 and K > 1 or nat.row_stride(a) % 16 or a.data_ptr() % 16):
+        raise ValueError(f"{name}: the rows must be 16-byte aligned with unit column stride (quantize_fp8_rows lays them out so)")
+    if not a_scale.t().is_contiguous():
+        a_scale = a_scale.t().contiguous().t()
+    return a_scale
+
+
+def _check_weight(name, w, w_scale, K, dev):
+    w3 = w if w.dim() == 3 else w.unsqueeze(0)
+    s3 = w_scale if w_scale.dim() == 3 else w_scale.unsqueeze(0)
+    if w3.dim() != 3 or w3.dtype != E4M3 or w3.shape[2] != K or w3.device != dev or min(w3.shape) < 1:
+        raise ValueError(f"{name}: the weight must be an e4m3 (N, {K}) or (G, N, {K}) on the rows' device")
+    G, N, _ = w3.shape
+    if s3.shape != (G, _blocks(N), _blocks(K)) or s3.dtype != torch.float32 or s3.device != dev:
+        raise ValueError(f"{name}: the weight's scales must be fp32 (.., ceil(N / 128), ceil(K / 128)) on the rows' device")
+    ldw = w3.stride(1) if N > 1 else -(-K // 16) * 16
+    if w3.stride(2) != 1 and K > 1 or ldw % 16 or ldw < K or (G > 1 and w3.stride(0) % 16) or w3.data_ptr() % 16:
+        raise ValueError(f"{name}: the weight's rows must be 16-byte aligned with unit column stride "
+                         "(quantize_fp8_weight lays them out so)")
+    return w3, s3.contiguous(), G, N, ldw
+
+
+def _check_offsets(name, offsets, G, dev):
+    if offsets is None:
+        if G != 1:
+            raise ValueError(f"{name}: {G} groups need offsets")
+    elif offsets.dtype != torch.int32 or offsets.numel() != G + 1 or not offsets.is_contiguous() or offsets.device != dev:
+        raise ValueError(f"{name}: offsets must be a contiguous int32 (G + 1,) tensor on the rows' device")
+
+
+def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+               offsets: torch.Tensor | None = None, *, relu_sq: bool = False, out_dtype: torch.dtype = torch.bfloat16,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """out[m] = a[m] @ w[g]^T for the rows m in [offsets[g], offsets[g + 1]), of the values that the
+    e4m3 operands and their scales stand for; fp32 accumulation, one rounding to ``out_dtype``.
+
+    a (M, K) with a_scale as :func:`quantize_fp8_rows` returns them, w (N, K) or (G, N, K) with w_scale
+    as :func:`quantize_fp8_weight` does.  ``offsets`` (G + 1,) int32 on the device, ascending, or None for
+    one group over all rows; rows outside every group are left as they were in ``out``.  ``relu_sq``:
+    relu(.)^2 of the fp32 product.  No gradient (see :func:`fp8_linear`)."""
+    a_scale = _check_rows("fp8_matmul", a, a_scale)
+    M, K = a.shape
+    dev = a.device
+    w3, s3, G, N, ldw = _check_weight("fp8_matmul", w, w_scale, K, dev)
+    _check_offsets("fp8_matmul", offsets, G, dev)
+    if out is None:
+        out = torch.empty((M, N), device=dev, dtype=out_dtype)
+    elif out.shape != (M, N) or (out.stride(1) != 1 and N > 1) or out.device != dev:
+        raise ValueError("fp8_matmul: out must be (M, N) on the rows' device with unit column stride")
+    L = nat.lib()
+    with nat.on_device(dev):
+        rc = L.rwkv_fp8_gemm(nat.ptr(a), nat.row_stride(a), nat.ptr(a_scale), nat.ptr(w3), ldw, w3.stride(0), nat.ptr(s3),
+                             nat.ptr(offsets), nat.ptr(out), nat.row_stride(out), M, N, K, G, int(relu_sq),
+                             nat.dtype_code(out), nat.stream_ptr(dev))
+    nat.check(rc, "rwkv_fp8_gemm")
+    return out
+
+
+def _linear(x2d, w, w_scale):
+    q, s = quantize_fp8_rows(x2d)
+    return fp8_matmul(q, s, w, w_scale, out_dtype=x2d.dtype)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x2d, w, w_scale, w_t, w_scale_t):
+        ctx.save_for_backward(w_t, w_scale_t)
+        return _linear(x2d, w, w_scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _linear(dy, *ctx.saved_tensors), None, None, None, None
+
+
+def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, w_t: torch.Tensor | None = None,
+               w_scale_t: torch.Tensor | None = None) -> torch.Tensor:
+    """x (..., K) @ w^T -> (..., N) in x's dtype: x is quantised in the call, w (N, K) is held in e4m3.
+
+    The weight is frozen.  For an x that requires grad, pass the transposed layout
+    (:func:`transpose_fp8_weight`, kept beside the weight): dx = q(dy) @ w runs on the same kernels,
+    with dy quantised like x."""
+    if w.dim() != 2:
+        raise ValueError("fp8_linear: w must be (N, K)")
+    if x.shape[-1] != w.shape[1]:
+        raise ValueError(f"fp8_linear: x has {x.shape[-1]} columns, the weight {w.shape[1]}")
+    x2 = nat.rows_2d(x)
+    if x.requires_grad and torch.is_grad_enabled():
+        if w_t is None or w_scale_t is None:
+            raise RuntimeError("fp8_linear: an input that requires grad needs the transposed weight "
+                               "(transpose_fp8_weight) for the gradient")
+        y = _Linear.apply(x2, w, w_scale, w_t, w_scale_t)
+    else:
+        y = _linear(x2, w, w_scale)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
+
+
+def fp8_experts(rows: torch.Tensor, key: torch.Tensor, key_scale: torch.Tensor, value: torch.Tensor,
+                value_scale: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """Each expert's squared-ReLU layer over its rows: value_e(q(relu(key_e(q(x)))^2)), in rows' dtype.
+
+    rows (M, C) sorted by expert, expert e owning [offsets[e], offsets[e + 1]); key (E, D, C) and
+    value (E, C, D) e4m3 with their scales.  Rows outside every expert are undefined.  Forward only."""
+    if torch.is_grad_enabled() and rows.requires_grad:
+        raise RuntimeError("fp8_experts: forward only; call it under torch.no_grad() or on rows without gradient")
+    q, s = quantize_fp8_rows(rows)
+    h = fp8_matmul(q, s, key, key_scale, offsets, relu_sq=True, out_dtype=torch.float32)
+    q, s = quantize_fp8_rows(h)
+    return fp8_matmul(q, s, value, value_scale, offsets, out_dtype=rows.dtype)
