@@ -358,6 +358,9 @@ int rwkv_quantize_fp8_weight(const void* w, void* q, long long ldq, float* scale
 int rwkv_fp8_gemm(const void* a, long long lda, const float* a_scale, const void* w, long long ldw,
                   long long w_group_stride, const float* w_scale, const int32_t* offs, void* out, long long ldo,
                   int M, int N, int K, int G, int epi, int out_dtype, void* stream);
+/* Select the kernel of rwkv_fp8_gemm: 0 automatic, 1 mma.sync (streams the weights, for few
+ * rows), 2 tcgen05.  Process-wide; meant for testing one against the other. */
+int rwkv_fp8_set_gemm_impl(int impl);
 
 /* sum_{i<j} ||A_i^T A_j||_F^2 over the expert down-projections
  * (LoRAMoE_CMix.orthogonal_loss, moe.py:149-163).  A (E, C, R) dtype;

@@ -75,6 +75,7 @@ SIGNATURES = {
     "rwkv_quantize_fp8_rows": (_I, [_P, _LL, _P, _LL, _P, _I, _I, _I, _P]),
     "rwkv_quantize_fp8_weight": (_I, [_P, _P, _LL, _P] + [_I] * 4 + [_P]),
     "rwkv_fp8_gemm": (_I, [_P, _LL, _P, _P, _LL, _LL, _P, _P, _P, _LL] + [_I] * 6 + [_P]),
+    "rwkv_fp8_set_gemm_impl": (_I, [_I]),
     "rwkv_grouped_gemm": (_I, [_P] * 4 + [_I] * 4 + [ctypes.c_longlong, _I, _I, _P]),
     "rwkv_head_ce_workspace_size": (_SZ, [_I, _I]),
     "rwkv_head_ce_stats": (_I, [_P] * 4 + [_I] * 3 + [_P, _SZ, _I, _P]),

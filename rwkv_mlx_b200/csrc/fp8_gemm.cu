@@ -118,7 +118,11 @@ int gemm_stream(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st) {
     return RWKV_ERR_DTYPE;
 }
 
-bool gemm_prefers_stream(int M, int N, int K, int G) { return true; }
+static int g_gemm_impl = 0;
+
+// Few rows: the weights are read once at most for every 32 rows of a group, and 16-row tiles
+// of W keep the SMs busy where 128 x 128 output tiles would not.
+static bool prefers_stream(int M, int G) { return M <= 32 || (G > 1 && (long long)M <= 8LL * G); }
 
 }  // namespace fp8
 }  // namespace rwkv
@@ -138,5 +142,13 @@ extern "C" int rwkv_fp8_gemm(const void* a, long long lda, const float* a_scale,
     if (!aligned(a, 16) || !aligned(w, 16) || lda % 16 || ldw % 16 || (G > 1 && w_group_stride % 16)) return RWKV_ERR_ALIGN;
     const fp8::GemmArgs p{(const uint8_t*)a, lda, a_scale, (const uint8_t*)w, ldw, w_group_stride, w_scale, offs, out, ldo,
                           nullptr, M, N, K, G};
-    return fp8::gemm_stream(p, epi, out_dtype, (cudaStream_t)stream);
+    const bool few = fp8::g_gemm_impl ? fp8::g_gemm_impl == 1 : fp8::prefers_stream(M, G);
+    return few ? fp8::gemm_stream(p, epi, out_dtype, (cudaStream_t)stream)
+               : fp8::gemm_tc(p, epi, out_dtype, (cudaStream_t)stream);
+}
+
+extern "C" int rwkv_fp8_set_gemm_impl(int impl) {
+    if (impl < 0 || impl > 2) return RWKV_ERR_ARG;
+    fp8::g_gemm_impl = impl;
+    return RWKV_OK;
 }

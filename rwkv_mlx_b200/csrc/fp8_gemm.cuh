@@ -23,7 +23,6 @@ struct GemmArgs {
 
 int gemm_stream(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st);
 int gemm_tc(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st);
-bool gemm_prefers_stream(int M, int N, int K, int G);
 
 }  // namespace fp8
 }  // namespace rwkv

@@ -1,0 +1,402 @@
+// e4m3 products on the 5th-generation tensor cores (tcgen05, kind::f8f6f4) with TMA:
+//
+//   out[m, n] = epi( sum_kb as[kb, m] ws[g, n / 128, kb] sum_{k in block kb} a[m, k] w[g, n, k] )
+//
+// The scales change with every 128 values of K, so tensor memory holds only one K block's
+// sum at a time: the MMA warp writes block kb's 128 x BN product into one of two
+// accumulators (no accumulation across blocks), and the drain warps add it, times the row's
+// and the weight block's scale, to fp32 sums in registers while the other accumulator is
+// being written.  128 bytes of K are exactly one 128-byte swizzle row, so a pipeline stage
+// is one scale block.
+//   warp 8 lane 0   producer: A (128 x 128) and W (BN x 128) boxes by TMA into a ring;
+//   warp 9 lane 0   MMA issuer (warps 10 and 11 only give up their registers): 4 MMAs (128 x BN x 32) per block, commits to the stage's
+//                   "empty" barrier and the accumulator's "full" barrier;
+//   warps 0-7       drain: TMEM lane 32 (w % 4) + l = row of the tile, warps w and w + 4 take
+//                   the two column halves; one scale product per row and block.
+// The squared-ReLU expert's hidden rows are quantised in the epilogue: a thread holds one
+// row's columns, so a block's maximum is its own (BN = 256) or shared by two threads
+// (BN = 128).
+// Every wait is bounded as in gemm_tc.cu: a wait that gives up sets the CTA's abort flag and
+// the device error word, the CTA's remaining outputs become NaN, copies and MMAs in flight
+// are drained before the tensor memory is freed.  No load uses cluster multicast.
+#include "fp8_gemm.cuh"
+#include "tma_common.cuh"
+#include "wkv7.cuh"
+
+namespace rwkv {
+
+__device__ int g_device_error_fp8;
+// Test hook (rwkv_debug_force_wait_timeout): every bounded wait gives up at once.
+static __constant__ int c_force_wait_timeout_fp8;
+
+namespace fp8 {
+using namespace tcc;
+using namespace tma;
+
+constexpr int BM = 128, NDRAIN = 256, NTH = NDRAIN + 128, MAXG = 256, CTRL = 4096;
+// A drain thread keeps BN / 2 sums and 32 loaded values, more than the 168 registers that 384
+// threads can have: the drain warpgroups take them from the third (setmaxnreg).
+constexpr int REG_LAUNCH = 168, REG_DRAIN = 216, REG_ISSUE = 72;
+static_assert(REG_DRAIN * NDRAIN + REG_ISSUE * (NTH - NDRAIN) <= REG_LAUNCH * NTH, "register split");
+
+struct Ctrl {
+    unsigned long long full[8], empty[8], acc_full[2], acc_empty[2], drain;
+    uint32_t tmem_base;
+    int abort;
+    int goff[MAXG + 1];   // row offsets of the groups
+    int gunit[MAXG + 1];  // first unit of every group; [G] = number of units
+    float amax[2][BM];    // RELU2_Q with BN = 128: the two halves' maxima of each row
+};
+static_assert(sizeof(Ctrl) <= CTRL, "control block");
+
+template <int BN>
+struct Cfg {
+    static constexpr int A_BYTES = BM * BLK, B_BYTES = BN * BLK, STAGE = A_BYTES + B_BYTES;
+    static constexpr int NS = BN == 256 ? 4 : 6;
+    static constexpr int SMEM = 1024 + CTRL + NS * STAGE;
+    static_assert(SMEM <= 227 * 1024 && NS <= 8, "shared memory");
+};
+
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int Nn) {  // fp32 accumulate, both e4m3, K-major
+    return (1u << 4) | ((uint32_t)(Nn >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void umma8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8}, p; }" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0), "r"(0), "r"(0), "r"(0)
+        : "memory");
+}
+__device__ __forceinline__ bool wait_f(unsigned long long* b, uint32_t parity, volatile int* abort) {
+    if (c_force_wait_timeout_fp8) {
+        *abort = 1;
+        atomicOr(&g_device_error_fp8, 2);
+        return false;
+    }
+    return ck::mbar_wait(b, parity, abort, &g_device_error_fp8);
+}
+
+struct Unit {
+    int g, row0, rend, nt;
+};
+__device__ __forceinline__ Unit unit_of(const Ctrl& cs, int G, int ntn, int u) {
+    int lo = 0, hi = G;  // largest g with gunit[g] <= u (empty groups repeat a value)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cs.gunit[mid] <= u) lo = mid;
+        else hi = mid;
+    }
+    const int l = u - cs.gunit[lo];
+    return {lo, cs.goff[lo] + l / ntn * BM, cs.goff[lo + 1], l % ntn};
+}
+
+template <int EPI, int HC, typename TO>
+__device__ __forceinline__ void store_row(const GemmArgs& p, float (&acc)[HC], int row, int n0, bool vec, float mul) {
+    const int ncol = p.N - n0;
+    if constexpr (EPI == RELU2_Q) {
+        uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + (long long)row * p.ldo + n0;
+#pragma unroll
+        for (int c = 0; c < HC; c += 16) {
+            uint4 r;
+            r.x = pack4(acc[c] * mul, acc[c + 1] * mul, acc[c + 2] * mul, acc[c + 3] * mul);
+            r.y = pack4(acc[c + 4] * mul, acc[c + 5] * mul, acc[c + 6] * mul, acc[c + 7] * mul);
+            r.z = pack4(acc[c + 8] * mul, acc[c + 9] * mul, acc[c + 10] * mul, acc[c + 11] * mul);
+            r.w = pack4(acc[c + 12] * mul, acc[c + 13] * mul, acc[c + 14] * mul, acc[c + 15] * mul);
+            if (vec && c + 16 <= ncol) {
+                *reinterpret_cast<uint4*>(o + c) = r;
+            } else {
+                const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (c + e < ncol) o[c + e] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+            }
+        }
+    } else {
+        constexpr int PER = 16 / sizeof(TO);
+        TO* o = reinterpret_cast<TO*>(p.out) + (long long)row * p.ldo + n0;
+#pragma unroll
+        for (int c = 0; c < HC; c += PER) {
+            alignas(16) TO r[PER];
+#pragma unroll
+            for (int e = 0; e < PER; e++) r[e] = from_f32<TO>(acc[c + e]);
+            if (vec && c + PER <= ncol) {
+                *reinterpret_cast<uint4*>(o + c) = *reinterpret_cast<uint4*>(r);
+            } else {
+#pragma unroll
+                for (int e = 0; e < PER; e++)
+                    if (c + e < ncol) o[c + e] = r[e];
+            }
+        }
+    }
+}
+
+}  // namespace fp8
+
+template <int BN, int EPI, typename TO>
+__global__ void __launch_bounds__(fp8::NTH, 1)
+    fp8_gemm_tc_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mw,
+                       const fp8::GemmArgs p, const int vec) {
+    using namespace fp8;
+    using C = Cfg<BN>;
+    constexpr int NS = C::NS, HC = BN / 2;
+    constexpr uint32_t IDESC = idesc_e4m3(BM, BN), TCOLS = 2 * BN;
+
+    extern __shared__ __align__(1024) unsigned char smem_fp8_raw[];
+    const uint32_t raw_addr = ck::smem_u32(smem_fp8_raw);
+    unsigned char* smem = smem_fp8_raw + (((raw_addr + 1023) & ~1023u) - raw_addr);
+    Ctrl& cs = *reinterpret_cast<Ctrl*>(smem);
+    unsigned char* ring = smem + CTRL;  // stage s: A box (16 KB) then W box (BN * 128 B), 1024-aligned
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int nk = (p.K + BLK - 1) / BLK, ntn = (p.N + BN - 1) / BN;
+
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ck::smem_u32(&cs.tmem_base)),
+                     "n"(TCOLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == NDRAIN) {
+        for (int i = 0; i < NS; i++) ck::mbar_init(&cs.full[i], 1), ck::mbar_init(&cs.empty[i], 1);
+        for (int i = 0; i < 2; i++) ck::mbar_init(&cs.acc_full[i], 1), ck::mbar_init(&cs.acc_empty[i], NDRAIN);
+        ck::mbar_init(&cs.drain, 1);
+        cs.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // offsets are clamped to [0, M]: rows outside the matrix belong to no tile
+    if (tid <= p.G) cs.goff[tid] = p.offs ? min(max(p.offs[tid], 0), p.M) : (tid == 0 ? 0 : p.M);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) {  // units per group (empty or negative groups: none), exclusive scan over the groups
+        constexpr int PER = (MAXG + 31) / 32;
+        int loc[PER], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int g = lane * PER + i;
+            const int rows = g < p.G ? cs.goff[g + 1] - cs.goff[g] : 0;
+            loc[i] = sum;
+            sum += rows > 0 ? (rows + BM - 1) / BM * ntn : 0;
+        }
+        int incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += t;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int g = lane * PER + i;
+            if (g < p.G) cs.gunit[g] = incl - sum + loc[i];
+        }
+        if (lane == 31) cs.gunit[p.G] = incl;
+    }
+    __syncthreads();
+    const uint32_t tmem = cs.tmem_base;
+    const int nunits = cs.gunit[p.G];
+
+    if (warp >= NDRAIN / 32) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_ISSUE));
+        if (warp == NDRAIN / 32) {
+            // ===================== producer =====================
+            if (lane == 0) {
+                int it = 0;
+                bool bad = false;
+                for (int u = blockIdx.x; u < nunits && !bad && !*(volatile int*)&cs.abort; u += gridDim.x) {
+                    const Unit un = unit_of(cs, p.G, ntn, u);
+                    for (int kb = 0; kb < nk; kb++, it++) {
+                        const int s = it % NS;
+                        if (it >= NS && !wait_f(&cs.empty[s], ((it / NS) + 1) & 1, &cs.abort)) {
+                            bad = true;
+                            break;
+                        }
+                        unsigned char* st = ring + s * C::STAGE;
+                        expect_tx(&cs.full[s], C::STAGE);
+                        tma_load_2d(st, &ma, kb * BLK, un.row0, &cs.full[s]);
+                        tma_load_3d(st + C::A_BYTES, &mw, kb * BLK, un.nt * BN, un.g, &cs.full[s]);
+                    }
+                }
+                // the last NS copies may still be in flight: the shared memory they write must
+                // stay allocated until they have landed
+                for (int i = (it > NS ? it - NS : 0); i < it; i++)
+                    ck::mbar_drain(&cs.full[i % NS], (i / NS) & 1, &g_device_error_fp8);
+            }
+            __syncwarp();
+        } else if (warp == NDRAIN / 32 + 1) {
+            // ===================== MMA issuer =====================
+            if (lane == 0) {
+                int it = 0;
+                bool bad = false;
+                for (int u = blockIdx.x; u < nunits && !bad && !*(volatile int*)&cs.abort; u += gridDim.x) {
+                    for (int kb = 0; kb < nk; kb++, it++) {
+                        const int s = it % NS, acc = it & 1;
+                        if ((it >= 2 && !wait_f(&cs.acc_empty[acc], ((it >> 1) + 1) & 1, &cs.abort)) ||
+                            !wait_f(&cs.full[s], (it / NS) & 1, &cs.abort)) {
+                            bad = true;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t sa = ck::smem_u32(ring + s * C::STAGE), sb = sa + C::A_BYTES;
+#pragma unroll
+                        for (int kk = 0; kk < BLK / 32; kk++)
+                            umma8(tmem + acc * BN, desc_sw128(sa + kk * 32, 16, 1024), desc_sw128(sb + kk * 32, 16, 1024),
+                                  IDESC, kk > 0 ? 1u : 0u);
+                        umma_commit(&cs.empty[s]);
+                        umma_commit(&cs.acc_full[acc]);
+                    }
+                }
+                if (it > 0) {  // wait for this thread's own MMAs before the memory is freed
+                    umma_commit(&cs.drain);
+                    ck::mbar_drain(&cs.drain, 0, &g_device_error_fp8);
+                }
+            }
+            __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_DRAIN));
+        // ===================== drain and epilogue =====================
+        const int ew = warp & 3, half = warp >> 2;
+        const int rl = 32 * ew + lane;  // row of the tile = TMEM lane
+        const uint32_t tl = tmem + ((uint32_t)(32 * ew) << 16) + half * HC;
+        const int nbn = (p.N + BLK - 1) / BLK;
+        bool ab = false;
+        int it = 0;
+        for (int u = blockIdx.x; u < nunits; u += gridDim.x) {
+            const Unit un = unit_of(cs, p.G, ntn, u);
+            const int row = un.row0 + rl, n0 = un.nt * BN + half * HC, nb = n0 / BLK;
+            const bool valid = row < un.rend;
+            const float* sap = p.as + row;
+            const float* sbp = p.ws + ((long long)un.g * nbn + (nb < nbn ? nb : nbn - 1)) * nk;
+            float acc[HC];
+#pragma unroll
+            for (int c = 0; c < HC; c++) acc[c] = 0.f;
+            float s_next = valid ? sap[0] * sbp[0] : 0.f;
+            for (int kb = 0; kb < nk; kb++, it++) {
+                const float s = s_next;
+                if (kb + 1 < nk) s_next = valid ? sap[(long long)(kb + 1) * p.M] * sbp[kb + 1] : 0.f;
+                const int b = it & 1;
+                if (!ab) ab = !wait_f(&cs.acc_full[b], (it >> 1) & 1, &cs.abort);
+                ab = __any_sync(0xffffffffu, ab);
+                if (ab) break;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < HC; c += 32) {
+                    float v[32];
+                    tmem_ld32(tl + b * BN + c, v);
+                    tmem_wait_ld();
+                    if (c + 32 == HC) {
+                        tc_fence_before();
+                        ck::mbar_arrive(&cs.acc_empty[b]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e++) acc[c + e] = fmaf(s, v[e], acc[c + e]);
+                }
+            }
+            if (ab) {
+#pragma unroll
+                for (int c = 0; c < HC; c++) acc[c] = __int_as_float(0x7fc00000);
+            }
+            if (EPI != STORE) {
+#pragma unroll
+                for (int c = 0; c < HC; c++) acc[c] = acc[c] > 0.f ? acc[c] * acc[c] : (acc[c] == acc[c] ? 0.f : acc[c]);
+            }
+            float mul = 1.f;
+            if (EPI == RELU2_Q) {
+                float a = 0.f;
+#pragma unroll
+                for (int c = 0; c < HC; c++) a = fmaxf(a, acc[c]);  // columns past N are 0
+                if (HC < BLK) {
+                    cs.amax[half][rl] = a;
+                    ck::bar_sync_n(1, NDRAIN);
+                    a = fmaxf(cs.amax[0][rl], cs.amax[1][rl]);
+                    ck::bar_sync_n(1, NDRAIN);
+                }
+                a = clamp_amax(a);
+                mul = quant_mul(a);
+                if (valid && n0 < p.N && n0 % BLK == 0) p.os[(long long)nb * p.M + row] = dequant_scale(a);
+            }
+            if (valid && n0 < p.N) store_row<EPI, HC, TO>(p, acc, row, n0, vec != 0, mul);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(TCOLS) : "memory");
+    }
+}
+
+namespace fp8 {
+
+static int sm_count() {
+    int dev = 0, n = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n;
+}
+
+template <int BN, int EPI, typename TO>
+static int launch_tc(const GemmArgs& p, int grid, cudaStream_t st) {
+    using C = Cfg<BN>;
+    alignas(64) CUtensorMap ma, mw;
+    {
+        const cuuint64_t dims[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M}, strides[1] = {(cuuint64_t)p.lda};
+        const cuuint32_t box[2] = {(cuuint32_t)BLK, (cuuint32_t)BM};
+        if (make_map_dt(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.a, 2, dims, strides, box, true)) return RWKV_ERR_CUDA;
+    }
+    {
+        const cuuint64_t dims[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.G};
+        const cuuint64_t strides[2] = {(cuuint64_t)p.ldw, (cuuint64_t)(p.G > 1 ? p.gsw : (long long)p.N * p.ldw)};
+        const cuuint32_t box[3] = {(cuuint32_t)BLK, (cuuint32_t)BN, 1};
+        if (make_map_dt(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, 3, dims, strides, box, true)) return RWKV_ERR_CUDA;
+    }
+    auto kern = fp8_gemm_tc_kernel<BN, EPI, TO>;
+    const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (err != cudaSuccess) return set_cuda_error(err);
+    const int vec = aligned(p.out, 16) && (p.ldo * (EPI == RELU2_Q ? 1 : (int)sizeof(TO))) % 16 == 0;
+    kern<<<grid, NTH, C::SMEM, st>>>(ma, mw, p, vec);
+    return check_launch();
+}
+
+template <int BN>
+static int by_epi(const GemmArgs& p, int epi, int out_dtype, int grid, cudaStream_t st) {
+    if (epi == RELU2_Q) return launch_tc<BN, RELU2_Q, uint8_t>(p, grid, st);
+    RWKV_DISPATCH_DTYPE(out_dtype, TO, {
+        return epi == RELU2 ? launch_tc<BN, RELU2, TO>(p, grid, st) : launch_tc<BN, STORE, TO>(p, grid, st);
+    });
+    return RWKV_ERR_DTYPE;
+}
+
+// An upper bound of the row tiles of all groups that needs no offsets.
+static long long row_tiles(int M, int G) {
+    const long long most = (M + BM - 1) / BM + (G > 1 ? G - 1 : 0);
+    return most < M ? most : M;
+}
+
+int gemm_tc(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st) {
+    const int sms = sm_count();
+    const long long mt = row_tiles(p.M, p.G), t256 = mt * ((p.N + 255) / 256), t128 = mt * ((p.N + 127) / 128);
+    if (t256 >= sms) return by_epi<256>(p, epi, out_dtype, (int)(t256 < sms ? t256 : sms), st);
+    return by_epi<128>(p, epi, out_dtype, (int)(t128 < sms ? t128 : sms), st);
+}
+
+}  // namespace fp8
+
+int read_device_error_fp8(int clear) {
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_device_error_fp8, sizeof(int));
+    if (e != cudaSuccess) return -set_cuda_error(e);
+    if (clear && v) {
+        const int z = 0;
+        e = cudaMemcpyToSymbol(g_device_error_fp8, &z, sizeof(int));
+        if (e != cudaSuccess) return -set_cuda_error(e);
+    }
+    return v;
+}
+int set_force_wait_timeout_fp8(int on) {
+    return set_cuda_error(cudaMemcpyToSymbol(c_force_wait_timeout_fp8, &on, sizeof(int)));
+}
+int set_device_error_fp8(int value) {
+    return set_cuda_error(cudaMemcpyToSymbol(g_device_error_fp8, &value, sizeof(int)));
+}
+
+}  // namespace rwkv

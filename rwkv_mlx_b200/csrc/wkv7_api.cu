@@ -103,13 +103,15 @@ extern "C" int rwkv_set_wkv_segments(int nseg) {
 }
 
 extern "C" int rwkv_debug_force_wait_timeout(int on) {
-    const int rc = set_force_wait_timeout_tc(on);
+    int rc = set_force_wait_timeout_tc(on);
+    if (!rc) rc = set_force_wait_timeout_fp8(on);
     return rc ? rc : set_force_wait_timeout_gemm(on);
 }
 
 extern "C" int rwkv_debug_set_device_error(int value) {
     int rc = set_device_error_tc(value);
     if (!rc) rc = set_device_error_bwd(value);
+    if (!rc) rc = set_device_error_fp8(value);
     return rc ? rc : set_device_error_gemm(value);
 }
 
