@@ -53,7 +53,7 @@ template <int BN>
 struct Cfg {
     static constexpr int A_BYTES = BM * BLK, B_BYTES = BN * BLK, STAGE = A_BYTES + B_BYTES;
     static constexpr int NS = BN == 256 ? 4 : 6;
-    static constexpr int SMEM = 1024 + CTRL + NS * STAGE;
+    static constexpr int SMEM = 1024 + CTRL + NS * STAGE + NDRAIN / 32 * 2048;
     static_assert(SMEM <= 227 * 1024 && NS <= 8, "shared memory");
 };
 
@@ -76,6 +76,14 @@ __device__ __forceinline__ bool wait_f(unsigned long long* b, uint32_t parity, v
     return ck::mbar_wait(b, parity, abort, &g_device_error_fp8);
 }
 
+// a0 += s * v[0], a1 += s * v[1] in one packed instruction (same roundings as two fmaf).
+__device__ __forceinline__ void fma2(float& a0, float& a1, const float* v, float s) {
+    asm("{ .reg .b64 a, b, c; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %4}; mov.b64 c, {%0, %1}; "
+        "fma.rn.f32x2 c, a, b, c; mov.b64 {%0, %1}, c; }"
+        : "+f"(a0), "+f"(a1)
+        : "f"(v[0]), "f"(v[1]), "f"(s));
+}
+
 struct Unit {
     int g, row0, rend, nt;
 };
@@ -90,43 +98,58 @@ __device__ __forceinline__ Unit unit_of(const Ctrl& cs, int G, int ntn, int u) {
     return {lo, cs.goff[lo] + l / ntn * BM, cs.goff[lo + 1], l % ntn};
 }
 
-template <int EPI, int HC, typename TO>
-__device__ __forceinline__ void store_row(const GemmArgs& p, float (&acc)[HC], int row, int n0, bool vec, float mul) {
-    const int ncol = p.N - n0;
+// 16 bytes of outputs from PER sums.
+template <int EPI, typename TO, int PER>
+__device__ __forceinline__ uint4 pack_out(const float* v, float mul) {
+    uint4 r;
     if constexpr (EPI == RELU2_Q) {
-        uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + (long long)row * p.ldo + n0;
-#pragma unroll
-        for (int c = 0; c < HC; c += 16) {
-            uint4 r;
-            r.x = pack4(acc[c] * mul, acc[c + 1] * mul, acc[c + 2] * mul, acc[c + 3] * mul);
-            r.y = pack4(acc[c + 4] * mul, acc[c + 5] * mul, acc[c + 6] * mul, acc[c + 7] * mul);
-            r.z = pack4(acc[c + 8] * mul, acc[c + 9] * mul, acc[c + 10] * mul, acc[c + 11] * mul);
-            r.w = pack4(acc[c + 12] * mul, acc[c + 13] * mul, acc[c + 14] * mul, acc[c + 15] * mul);
-            if (vec && c + 16 <= ncol) {
-                *reinterpret_cast<uint4*>(o + c) = r;
-            } else {
-                const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    if (c + e < ncol) o[c + e] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
-            }
-        }
+        r.x = pack4(v[0] * mul, v[1] * mul, v[2] * mul, v[3] * mul);
+        r.y = pack4(v[4] * mul, v[5] * mul, v[6] * mul, v[7] * mul);
+        r.z = pack4(v[8] * mul, v[9] * mul, v[10] * mul, v[11] * mul);
+        r.w = pack4(v[12] * mul, v[13] * mul, v[14] * mul, v[15] * mul);
     } else {
-        constexpr int PER = 16 / sizeof(TO);
-        TO* o = reinterpret_cast<TO*>(p.out) + (long long)row * p.ldo + n0;
+        TO* o = reinterpret_cast<TO*>(&r);
 #pragma unroll
-        for (int c = 0; c < HC; c += PER) {
-            alignas(16) TO r[PER];
+        for (int e = 0; e < PER; e++) o[e] = from_f32<TO>(v[e]);
+    }
+    return r;
+}
+
+// A warp's 32 rows x HC columns to memory.  A lane holds one row, so stores straight from
+// registers would write 16 bytes of 32 rows at a time (measured: 16,000 cycles for a 128 x 256
+// tile of 16-bit outputs, four times its products at K = 1024).  The warp turns 64-byte pieces
+// of its rows in 2 KB of its own shared memory (chunks permuted so that neither side has bank
+// conflicts) and stores 8 rows x 64 contiguous bytes at a time.
+template <int EPI, int HC, typename TO>
+__device__ __forceinline__ void store_rows(const GemmArgs& p, const float (&acc)[HC], unsigned char* buf, int row0,
+                                           int nrows, int n0, bool vec, float mul) {
+    constexpr int PER = 16 / sizeof(TO), CC = 4 * PER;  // outputs in 16 and in 64 bytes
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-            for (int e = 0; e < PER; e++) r[e] = from_f32<TO>(acc[c + e]);
-            if (vec && c + PER <= ncol) {
-                *reinterpret_cast<uint4*>(o + c) = *reinterpret_cast<uint4*>(r);
-            } else {
+    for (int c0 = 0; c0 < HC; c0 += CC) {
 #pragma unroll
-                for (int e = 0; e < PER; e++)
-                    if (c + e < ncol) o[c + e] = r[e];
+        for (int q = 0; q < 4; q++)
+            *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ (lane >> 1)) & 3) * 16) =
+                pack_out<EPI, TO, PER>(&acc[c0 + q * PER], mul);
+        __syncwarp();
+        const int q = lane & 3, n = n0 + c0 + q * PER;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = i * 8 + (lane >> 2);
+            const uint4 v = *reinterpret_cast<const uint4*>(buf + r * 64 + ((q ^ (r >> 1)) & 3) * 16);
+            if (r < nrows && n < p.N) {
+                TO* o = reinterpret_cast<TO*>(p.out) + (long long)(row0 + r) * p.ldo + n;
+                if (vec && n + PER <= p.N) {
+                    *reinterpret_cast<uint4*>(o) = v;
+                } else {
+                    const TO* e = reinterpret_cast<const TO*>(&v);
+#pragma unroll
+                    for (int j = 0; j < PER; j++)
+                        if (n + j < p.N) o[j] = e[j];
+                }
             }
         }
+        __syncwarp();
     }
 }
 
@@ -157,7 +180,7 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
     }
     if (tid == NDRAIN) {
         for (int i = 0; i < NS; i++) ck::mbar_init(&cs.full[i], 1), ck::mbar_init(&cs.empty[i], 1);
-        for (int i = 0; i < 2; i++) ck::mbar_init(&cs.acc_full[i], 1), ck::mbar_init(&cs.acc_empty[i], NDRAIN);
+        for (int i = 0; i < 2; i++) ck::mbar_init(&cs.acc_full[i], 1), ck::mbar_init(&cs.acc_empty[i], NDRAIN / 32);
         ck::mbar_init(&cs.drain, 1);
         cs.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -260,35 +283,71 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
         const int nbn = (p.N + BLK - 1) / BLK;
         bool ab = false;
         int it = 0;
+        // Scales come from L2 with a latency of one to two blocks' products, so they are loaded
+        // PF blocks at a time, one group of blocks ahead (and a unit's first group before the
+        // previous unit's outputs are stored).
+        constexpr int PF = 2;
+        float sa[PF], sb[PF];
+        const float *sap = nullptr, *sbp = nullptr;
+        auto aim = [&](const Unit& un) {
+            const int row = un.row0 + rl, nb = min((un.nt * BN + half * HC) / BLK, nbn - 1);
+            sap = row < un.rend ? p.as + row : nullptr;
+            sbp = p.ws + ((long long)un.g * nbn + nb) * nk;
+        };
+        auto fetch = [&](int kb0) {
+#pragma unroll
+            for (int i = 0; i < PF; i++) {
+                const bool on = kb0 + i < nk;
+                sa[i] = on && sap ? __ldg(sap + (long long)(kb0 + i) * p.M) : 0.f;
+                sb[i] = on ? __ldg(sbp + kb0 + i) : 0.f;
+            }
+        };
+        if ((int)blockIdx.x < nunits) {
+            aim(unit_of(cs, p.G, ntn, blockIdx.x));
+            fetch(0);
+        }
         for (int u = blockIdx.x; u < nunits; u += gridDim.x) {
             const Unit un = unit_of(cs, p.G, ntn, u);
             const int row = un.row0 + rl, n0 = un.nt * BN + half * HC, nb = n0 / BLK;
             const bool valid = row < un.rend;
-            const float* sap = p.as + row;
-            const float* sbp = p.ws + ((long long)un.g * nbn + (nb < nbn ? nb : nbn - 1)) * nk;
             float acc[HC];
 #pragma unroll
             for (int c = 0; c < HC; c++) acc[c] = 0.f;
-            float s_next = valid ? sap[0] * sbp[0] : 0.f;
-            for (int kb = 0; kb < nk; kb++, it++) {
-                const float s = s_next;
-                if (kb + 1 < nk) s_next = valid ? sap[(long long)(kb + 1) * p.M] * sbp[kb + 1] : 0.f;
-                const int b = it & 1;
-                if (!ab) ab = !wait_f(&cs.acc_full[b], (it >> 1) & 1, &cs.abort);
-                ab = __any_sync(0xffffffffu, ab);
-                if (ab) break;
-                tc_fence_after();
+            for (int kb0 = 0; kb0 < nk && !ab; kb0 += PF) {
+                float s[PF];
 #pragma unroll
-                for (int c = 0; c < HC; c += 32) {
-                    float v[32];
-                    tmem_ld32(tl + b * BN + c, v);
-                    tmem_wait_ld();
-                    if (c + 32 == HC) {
-                        tc_fence_before();
-                        ck::mbar_arrive(&cs.acc_empty[b]);
+                for (int i = 0; i < PF; i++) s[i] = sa[i] * sb[i];
+                if (kb0 + PF < nk) {
+                    fetch(kb0 + PF);
+                } else if (u + (int)gridDim.x < nunits) {
+                    aim(unit_of(cs, p.G, ntn, u + gridDim.x));
+                    fetch(0);
+                }
+#pragma unroll
+                for (int i = 0; i < PF; i++) {
+                    if (kb0 + i >= nk || ab) break;
+                    const int b = it & 1;
+                    ab = !wait_f(&cs.acc_full[b], (it >> 1) & 1, &cs.abort);
+                    ab = __any_sync(0xffffffffu, ab);
+                    if (ab) break;
+                    it++;
+                    tc_fence_after();
+                    const uint32_t at = tl + b * BN;
+                    float v[2][16];  // the next 16 columns load while these are added
+                    tmem_ld16(at, v[0]);
+#pragma unroll
+                    for (int c = 0; c < HC; c += 16) {
+                        tmem_wait_ld();
+                        if (c + 16 < HC) {
+                            tmem_ld16(at + c + 16, v[(c / 16 + 1) & 1]);
+                        } else {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) ck::mbar_arrive(&cs.acc_empty[b]);  // one arrival a warp: they serialise
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) fma2(acc[c + e], acc[c + e + 1], v[(c / 16) & 1] + e, s[i]);
                     }
-#pragma unroll
-                    for (int e = 0; e < 32; e++) acc[c + e] = fmaf(s, v[e], acc[c + e]);
                 }
             }
             if (ab) {
@@ -314,7 +373,9 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
                 mul = quant_mul(a);
                 if (valid && n0 < p.N && n0 % BLK == 0) p.os[(long long)nb * p.M + row] = dequant_scale(a);
             }
-            if (valid && n0 < p.N) store_row<EPI, HC, TO>(p, acc, row, n0, vec != 0, mul);
+            if (n0 < p.N)
+                store_rows<EPI, HC, TO>(p, acc, ring + NS * C::STAGE + warp * 2048, un.row0 + 32 * ew,
+                                        un.rend - un.row0 - 32 * ew, n0, vec != 0, mul);
         }
     }
 
