@@ -67,15 +67,16 @@ __device__ __forceinline__ void umma8(uint32_t d, uint64_t a, uint64_t b, uint32
         "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0), "r"(0), "r"(0), "r"(0)
         : "memory");
 }
+// Bounded wait; the first look is a bare try_wait, since the issuing thread's own instructions
+// are what bounds short blocks.
 __device__ __forceinline__ bool wait_f(unsigned long long* b, uint32_t parity, volatile int* abort) {
-    if (c_force_wait_timeout_fp8) {
-        *abort = 1;
-        atomicOr(&g_device_error_fp8, 2);
-        return false;
-    }
-    return ck::mbar_wait(b, parity, abort, &g_device_error_fp8);
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok)
+                 : "r"(ck::smem_u32(b)), "r"(parity)
+                 : "memory");
+    return ok || ck::mbar_wait(b, parity, abort, &g_device_error_fp8);
 }
-
 // a0 += s * v[0], a1 += s * v[1] in one packed instruction (same roundings as two fmaf).
 __device__ __forceinline__ void fma2(float& a0, float& a1, const float* v, float s) {
     asm("{ .reg .b64 a, b, c; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %4}; mov.b64 c, {%0, %1}; "
@@ -182,7 +183,8 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
         for (int i = 0; i < NS; i++) ck::mbar_init(&cs.full[i], 1), ck::mbar_init(&cs.empty[i], 1);
         for (int i = 0; i < 2; i++) ck::mbar_init(&cs.acc_full[i], 1), ck::mbar_init(&cs.acc_empty[i], NDRAIN / 32);
         ck::mbar_init(&cs.drain, 1);
-        cs.abort = 0;
+        cs.abort = c_force_wait_timeout_fp8 ? 1 : 0;
+        if (cs.abort) atomicOr(&g_device_error_fp8, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // offsets are clamped to [0, M]: rows outside the matrix belong to no tile
@@ -247,24 +249,27 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
         } else if (warp == NDRAIN / 32 + 1) {
             // ===================== MMA issuer =====================
             if (lane == 0) {
-                int it = 0;
+                // a descriptor's address field is bytes / 16 below 2^14: stages and K steps are added to it
+                const uint64_t desc_a = desc_sw128(ck::smem_u32(ring), 16, 1024);
+                int it = 0, s = 0;
+                uint32_t ph = 0;
                 bool bad = false;
                 for (int u = blockIdx.x; u < nunits && !bad && !*(volatile int*)&cs.abort; u += gridDim.x) {
                     for (int kb = 0; kb < nk; kb++, it++) {
-                        const int s = it % NS, acc = it & 1;
-                        if ((it >= 2 && !wait_f(&cs.acc_empty[acc], ((it >> 1) + 1) & 1, &cs.abort)) ||
-                            !wait_f(&cs.full[s], (it / NS) & 1, &cs.abort)) {
+                        const int acc = it & 1;
+                        if (!wait_f(&cs.full[s], ph, &cs.abort) ||
+                            (it >= 2 && !wait_f(&cs.acc_empty[acc], ((it >> 1) + 1) & 1, &cs.abort))) {
                             bad = true;
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t sa = ck::smem_u32(ring + s * C::STAGE), sb = sa + C::A_BYTES;
+                        const uint64_t da = desc_a + s * (C::STAGE >> 4);
 #pragma unroll
                         for (int kk = 0; kk < BLK / 32; kk++)
-                            umma8(tmem + acc * BN, desc_sw128(sa + kk * 32, 16, 1024), desc_sw128(sb + kk * 32, 16, 1024),
-                                  IDESC, kk > 0 ? 1u : 0u);
+                            umma8(tmem + acc * BN, da + kk * 2, da + (C::A_BYTES >> 4) + kk * 2, IDESC, kk > 0 ? 1u : 0u);
                         umma_commit(&cs.empty[s]);
                         umma_commit(&cs.acc_full[acc]);
+                        if (++s == NS) s = 0, ph ^= 1;
                     }
                 }
                 if (it > 0) {  // wait for this thread's own MMAs before the memory is freed
@@ -281,7 +286,7 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
         const int rl = 32 * ew + lane;  // row of the tile = TMEM lane
         const uint32_t tl = tmem + ((uint32_t)(32 * ew) << 16) + half * HC;
         const int nbn = (p.N + BLK - 1) / BLK;
-        bool ab = false;
+        bool ab = *(volatile int*)&cs.abort != 0;
         int it = 0;
         // Scales come from L2 with a latency of one to two blocks' products, so they are loaded
         // PF blocks at a time, one group of blocks ahead (and a unit's first group before the
