@@ -349,15 +349,31 @@ int rwkv_route_experts_backward(const void* logits, long long ld, const int32_t*
  *   with fp32 sums; a (M, K) pitch lda, w (G, N, K) pitch ldw and group pitch
  *   w_group_stride, all in bytes and multiples of 16 on 16-byte aligned bases; G <= 256;
  *   offs (G + 1) ascending int32 on the device, or NULL with G = 1.  out (M, N), row
- *   pitch ldo elements, in out_dtype; epi 0: the product, epi 1: relu(.)^2 of it.  Rows
- *   outside every group are not written.  M = 0 is valid. */
+ *   pitch ldo elements, in out_dtype; epi 0: the product, epi 1: relu(.)^2 of it,
+ *   epi 2: relu(.)^2 quantised like rows, out bytes and out_scale (ceil(N / 128), M)
+ *   (out_dtype unused; out_scale NULL otherwise).  Rows outside every group are not
+ *   written.  M = 0 is valid.
+ * rwkv_fp8_linear: out (M, N) = x w^T in dtype with x (M, K) in dtype quantised in the
+ *   call, through a 256-byte aligned workspace of rwkv_fp8_linear_workspace_size bytes.
+ * rwkv_fp8_experts: x (M, C) sorted by expert -> out (M, C) = the value product (val
+ *   (E, C, D)) of the quantised relu(.)^2 of the key product (key (E, D, C)) of the
+ *   quantised x, both in dtype; workspace 256-byte aligned. */
 int rwkv_quantize_fp8_rows(const void* x, long long ldx, void* q, long long ldq, float* scale, int M, int K,
                            int dtype, void* stream);
 int rwkv_quantize_fp8_weight(const void* w, void* q, long long ldq, float* scale, int G, int N, int K, int dtype,
                              void* stream);
 int rwkv_fp8_gemm(const void* a, long long lda, const float* a_scale, const void* w, long long ldw,
                   long long w_group_stride, const float* w_scale, const int32_t* offs, void* out, long long ldo,
-                  int M, int N, int K, int G, int epi, int out_dtype, void* stream);
+                  float* out_scale, int M, int N, int K, int G, int epi, int out_dtype, void* stream);
+size_t rwkv_fp8_linear_workspace_size(int M, int K);
+int rwkv_fp8_linear(const void* x, long long ldx, const void* w, long long ldw, const float* w_scale, void* out,
+                    long long ldo, void* workspace, size_t workspace_bytes, int M, int N, int K, int dtype,
+                    void* stream);
+size_t rwkv_fp8_experts_workspace_size(int M, int C, int D, int E);
+int rwkv_fp8_experts(const void* x, long long ldx, const void* key, long long ldk, long long key_group_stride,
+                     const float* key_scale, const void* val, long long ldv, long long val_group_stride,
+                     const float* val_scale, const int32_t* offs, void* out, long long ldo, void* workspace,
+                     size_t workspace_bytes, int M, int C, int D, int E, int dtype, void* stream);
 /* Select the kernel of rwkv_fp8_gemm: 0 automatic, 1 mma.sync (streams the weights, for few
  * rows), 2 tcgen05.  Process-wide; meant for testing one against the other. */
 int rwkv_fp8_set_gemm_impl(int impl);

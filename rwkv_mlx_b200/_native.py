@@ -74,7 +74,11 @@ SIGNATURES = {
     "rwkv_route_experts_backward": (_I, [_P, _LL] + [_P] * 4 + [_I] * 5 + [_F, _I, _P]),
     "rwkv_quantize_fp8_rows": (_I, [_P, _LL, _P, _LL, _P, _I, _I, _I, _P]),
     "rwkv_quantize_fp8_weight": (_I, [_P, _P, _LL, _P] + [_I] * 4 + [_P]),
-    "rwkv_fp8_gemm": (_I, [_P, _LL, _P, _P, _LL, _LL, _P, _P, _P, _LL] + [_I] * 6 + [_P]),
+    "rwkv_fp8_gemm": (_I, [_P, _LL, _P, _P, _LL, _LL, _P, _P, _P, _LL, _P] + [_I] * 6 + [_P]),
+    "rwkv_fp8_linear_workspace_size": (_SZ, [_I, _I]),
+    "rwkv_fp8_linear": (_I, [_P, _LL, _P, _LL, _P, _P, _LL, _P, _SZ] + [_I] * 4 + [_P]),
+    "rwkv_fp8_experts_workspace_size": (_SZ, [_I] * 4),
+    "rwkv_fp8_experts": (_I, [_P, _LL, _P, _LL, _LL, _P, _P, _LL, _LL, _P, _P, _P, _LL, _P, _SZ] + [_I] * 5 + [_P]),
     "rwkv_fp8_set_gemm_impl": (_I, [_I]),
     "rwkv_grouped_gemm": (_I, [_P] * 4 + [_I] * 4 + [ctypes.c_longlong, _I, _I, _P]),
     "rwkv_head_ce_workspace_size": (_SZ, [_I, _I]),
@@ -127,10 +131,16 @@ def load(path: Path | None = None) -> ctypes.CDLL:
     return _lib
 
 
+_has_gpu = False
+
+
 def lib() -> ctypes.CDLL:
-    if not torch.cuda.is_available():
-        raise RwkvNativeError("rwkv_mlx_b200 kernels need a CUDA device (no CPU fallback)")
-    return load()
+    global _has_gpu
+    if not _has_gpu:  # asked until the first yes: the question costs more than a small kernel's launch
+        if not torch.cuda.is_available():
+            raise RwkvNativeError("rwkv_mlx_b200 kernels need a CUDA device (no CPU fallback)")
+        _has_gpu = True
+    return _lib if _lib is not None else load()
 
 
 # Kernel launches issued through this binding (per C-ABI entry point: the number of
@@ -143,7 +153,7 @@ KERNELS_PER_CALL = {
     "rwkv_tmix_post": 1, "rwkv_relu_sq": 1, "rwkv_lora_act": 1, "rwkv_argmax_rows": 1, "rwkv_add_layernorm": 1, "rwkv_moe_expert_mix_rows": 1,
     "rwkv_ce_chunk": 1, "rwkv_ce_finalize": 1, "rwkv_ce_chunk_grad": 1,
     "rwkv_route_experts": 1, "rwkv_route_experts_backward": 1, "rwkv_quantize_fp8_rows": 1, "rwkv_quantize_fp8_weight": 1,
-    "rwkv_fp8_gemm": 1,
+    "rwkv_fp8_gemm": 1, "rwkv_fp8_linear": 2, "rwkv_fp8_experts": 3,
     "rwkv_grouped_gemm": 1, "rwkv_head_ce_stats": 2, "rwkv_head_ce_grad": 1,
 }
 launch_count = 0
@@ -161,11 +171,11 @@ def check(rc: int, what: str, kernels: int | None = None) -> None:
 
 
 def ptr(t: torch.Tensor | None):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def stream_ptr(device=None):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def on_device(dev: torch.device):

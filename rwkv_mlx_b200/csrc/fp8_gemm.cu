@@ -129,22 +129,113 @@ static bool prefers_stream(int M, int G) { return M <= 32 || (G > 1 && (long lon
 
 using namespace rwkv;
 
+namespace {
+
+using fp8::GemmArgs;
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+long long pitch16(long long k) { return (k + 15) / 16 * 16; }
+size_t rows_bytes(int M, int K) { return align256((size_t)M * pitch16(K)); }
+size_t scale_bytes(int M, int K) { return align256((size_t)M * ((K + fp8::BLK - 1) / fp8::BLK) * sizeof(float)); }
+
+int check_weight(const void* w, long long ldw, long long gs, const float* ws, int G, int N, int K) {
+    if (N <= 0 || K <= 0 || G <= 0 || G > 256) return RWKV_ERR_SHAPE;
+    if (ldw < K || (G > 1 && gs < (long long)(N - 1) * ldw + K)) return RWKV_ERR_SHAPE;
+    if (!w || !ws) return RWKV_ERR_ARG;
+    if (!aligned(w, 16) || ldw % 16 || (G > 1 && gs % 16)) return RWKV_ERR_ALIGN;
+    return RWKV_OK;
+}
+bool known(int dtype) { return dtype == RWKV_F32 || dtype == RWKV_F16 || dtype == RWKV_BF16; }
+
+int gemm(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st) {
+    const bool few = epi != fp8::RELU2_Q && (fp8::g_gemm_impl ? fp8::g_gemm_impl == 1 : fp8::prefers_stream(p.M, p.G));
+    return few ? fp8::gemm_stream(p, epi, out_dtype, st) : fp8::gemm_tc(p, epi, out_dtype, st);
+}
+
+}  // namespace
+
 extern "C" int rwkv_fp8_gemm(const void* a, long long lda, const float* a_scale, const void* w, long long ldw,
                              long long w_group_stride, const float* w_scale, const int32_t* offs, void* out,
-                             long long ldo, int M, int N, int K, int G, int epi, int out_dtype, void* stream) {
-    if (out_dtype != RWKV_F32 && out_dtype != RWKV_F16 && out_dtype != RWKV_BF16) return RWKV_ERR_DTYPE;
-    if (M < 0 || N <= 0 || K <= 0 || G <= 0 || G > 256) return RWKV_ERR_SHAPE;
-    if (lda < K || ldw < K || ldo < N || (G > 1 && w_group_stride < (long long)(N - 1) * ldw + K)) return RWKV_ERR_SHAPE;
-    if (epi != fp8::STORE && epi != fp8::RELU2) return RWKV_ERR_ARG;
+                             long long ldo, float* out_scale, int M, int N, int K, int G, int epi, int out_dtype,
+                             void* stream) {
+    if (epi != fp8::STORE && epi != fp8::RELU2 && epi != fp8::RELU2_Q) return RWKV_ERR_ARG;
+    if (epi != fp8::RELU2_Q && !known(out_dtype)) return RWKV_ERR_DTYPE;
+    if (M < 0 || lda < K || ldo < N) return RWKV_ERR_SHAPE;
+    const int rc = check_weight(w, ldw, w_group_stride, w_scale, G, N, K);
+    if (rc) return rc;
     if (G > 1 && !offs) return RWKV_ERR_ARG;
     if (M == 0) return RWKV_OK;
-    if (!a || !a_scale || !w || !w_scale || !out) return RWKV_ERR_ARG;
-    if (!aligned(a, 16) || !aligned(w, 16) || lda % 16 || ldw % 16 || (G > 1 && w_group_stride % 16)) return RWKV_ERR_ALIGN;
-    const fp8::GemmArgs p{(const uint8_t*)a, lda, a_scale, (const uint8_t*)w, ldw, w_group_stride, w_scale, offs, out, ldo,
-                          nullptr, M, N, K, G};
-    const bool few = fp8::g_gemm_impl ? fp8::g_gemm_impl == 1 : fp8::prefers_stream(M, G);
-    return few ? fp8::gemm_stream(p, epi, out_dtype, (cudaStream_t)stream)
-               : fp8::gemm_tc(p, epi, out_dtype, (cudaStream_t)stream);
+    if (!a || !a_scale || !out || (epi == fp8::RELU2_Q && !out_scale)) return RWKV_ERR_ARG;
+    if (!aligned(a, 16) || lda % 16) return RWKV_ERR_ALIGN;
+    return gemm({(const uint8_t*)a, lda, a_scale, (const uint8_t*)w, ldw, w_group_stride, w_scale, offs, out, ldo,
+                 out_scale, M, N, K, G},
+                epi, out_dtype, (cudaStream_t)stream);
+}
+
+extern "C" size_t rwkv_fp8_linear_workspace_size(int M, int K) {
+    return M <= 0 || K <= 0 ? 0 : rows_bytes(M, K) + scale_bytes(M, K);
+}
+
+extern "C" int rwkv_fp8_linear(const void* x, long long ldx, const void* w, long long ldw, const float* w_scale,
+                               void* out, long long ldo, void* workspace, size_t workspace_bytes, int M, int N, int K,
+                               int dtype, void* stream) {
+    if (!known(dtype)) return RWKV_ERR_DTYPE;
+    if (M < 0 || ldx < K || ldo < N) return RWKV_ERR_SHAPE;
+    int rc = check_weight(w, ldw, 0, w_scale, 1, N, K);
+    if (rc) return rc;
+    if (M == 0) return RWKV_OK;
+    if (!x || !out || !workspace) return RWKV_ERR_ARG;
+    if (!aligned(workspace, 256)) return RWKV_ERR_ALIGN;
+    if (workspace_bytes < rwkv_fp8_linear_workspace_size(M, K)) return RWKV_ERR_WORKSPACE;
+    uint8_t* q = (uint8_t*)workspace;
+    float* qs = (float*)(q + rows_bytes(M, K));
+    rc = rwkv_quantize_fp8_rows(x, ldx, q, pitch16(K), qs, M, K, dtype, stream);
+    if (rc) return rc;
+    return gemm({q, pitch16(K), qs, (const uint8_t*)w, ldw, 0, w_scale, nullptr, out, ldo, nullptr, M, N, K, 1},
+                fp8::STORE, dtype, (cudaStream_t)stream);
+}
+
+extern "C" size_t rwkv_fp8_experts_workspace_size(int M, int C, int D, int E) {
+    if (M <= 0 || C <= 0 || D <= 0 || E <= 0) return 0;
+    const size_t h = fp8::prefers_stream(M, E) || fp8::g_gemm_impl == 1 ? align256((size_t)M * D * sizeof(float)) : 0;
+    return rows_bytes(M, C) + scale_bytes(M, C) + rows_bytes(M, D) + scale_bytes(M, D) + h;
+}
+
+extern "C" int rwkv_fp8_experts(const void* x, long long ldx, const void* key, long long ldk, long long key_gs,
+                                const float* key_scale, const void* val, long long ldv, long long val_gs,
+                                const float* val_scale, const int32_t* offs, void* out, long long ldo, void* workspace,
+                                size_t workspace_bytes, int M, int C, int D, int E, int dtype, void* stream) {
+    if (!known(dtype)) return RWKV_ERR_DTYPE;
+    if (M < 0 || ldx < C || ldo < C) return RWKV_ERR_SHAPE;
+    int rc = check_weight(key, ldk, key_gs, key_scale, E, D, C);
+    if (!rc) rc = check_weight(val, ldv, val_gs, val_scale, E, C, D);
+    if (rc) return rc;
+    if (E > 1 && !offs) return RWKV_ERR_ARG;
+    if (M == 0) return RWKV_OK;
+    if (!x || !out || !workspace) return RWKV_ERR_ARG;
+    if (!aligned(workspace, 256)) return RWKV_ERR_ALIGN;
+    if (workspace_bytes < rwkv_fp8_experts_workspace_size(M, C, D, E)) return RWKV_ERR_WORKSPACE;
+    uint8_t* at = (uint8_t*)workspace;
+    auto take = [&](size_t n) { return at += n, at - n; };
+    uint8_t* q = take(rows_bytes(M, C));
+    float* qs = (float*)take(scale_bytes(M, C));
+    uint8_t* hq = take(rows_bytes(M, D));
+    float* hs = (float*)take(scale_bytes(M, D));
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool few = fp8::g_gemm_impl ? fp8::g_gemm_impl == 1 : fp8::prefers_stream(M, E);
+    rc = rwkv_quantize_fp8_rows(x, ldx, q, pitch16(C), qs, M, C, dtype, stream);
+    if (rc) return rc;
+    GemmArgs p{q, pitch16(C), qs, (const uint8_t*)key, ldk, key_gs, key_scale, offs, hq, pitch16(D), hs, M, D, C, E};
+    if (few) {  // 16 columns a CTA: a block's maximum is not in one place, so the hidden rows pass through fp32
+        p.out = at, p.ldo = D, p.os = nullptr;
+        rc = gemm(p, fp8::RELU2, RWKV_F32, st);
+        if (!rc) rc = rwkv_quantize_fp8_rows(at, D, hq, pitch16(D), hs, M, D, RWKV_F32, stream);
+    } else {
+        rc = gemm(p, fp8::RELU2_Q, dtype, st);
+    }
+    if (rc) return rc;
+    return gemm({hq, pitch16(D), hs, (const uint8_t*)val, ldv, val_gs, val_scale, offs, out, ldo, nullptr, M, C, D, E},
+                fp8::STORE, dtype, st);
 }
 
 extern "C" int rwkv_fp8_set_gemm_impl(int impl) {

@@ -122,6 +122,22 @@ def _check_offsets(name, offsets, G, dev):
         raise ValueError(f"{name}: offsets must be a contiguous int32 (G + 1,) tensor on the rows' device")
 
 
+def _gemm(name, a, a_scale, w, w_scale, offsets, out, out_scale, epi, out_code):
+    a_scale = _check_rows(name, a, a_scale)
+    M, K = a.shape
+    dev = a.device
+    w3, s3, G, N, ldw = _check_weight(name, w, w_scale, K, dev)
+    _check_offsets(name, offsets, G, dev)
+    if out.shape != (M, N) or (out.stride(1) != 1 and N > 1) or out.device != dev:
+        raise ValueError(f"{name}: out must be (M, N) on the rows' device with unit column stride")
+    L = nat.lib()
+    with nat.on_device(dev):
+        rc = L.rwkv_fp8_gemm(nat.ptr(a), nat.row_stride(a), nat.ptr(a_scale), nat.ptr(w3), ldw, w3.stride(0), nat.ptr(s3),
+                             nat.ptr(offsets), nat.ptr(out), nat.row_stride(out), nat.ptr(out_scale), M, N, K, G, epi,
+                             out_code, nat.stream_ptr(dev))
+    nat.check(rc, "rwkv_fp8_gemm")
+
+
 def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
                offsets: torch.Tensor | None = None, *, relu_sq: bool = False, out_dtype: torch.dtype = torch.bfloat16,
                out: torch.Tensor | None = None) -> torch.Tensor:
@@ -132,27 +148,43 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
     as :func:`quantize_fp8_weight` does.  ``offsets`` (G + 1,) int32 on the device, ascending, or None for
     one group over all rows; rows outside every group are left as they were in ``out``.  ``relu_sq``:
     relu(.)^2 of the fp32 product.  No gradient (see :func:`fp8_linear`)."""
-    a_scale = _check_rows("fp8_matmul", a, a_scale)
-    M, K = a.shape
-    dev = a.device
-    w3, s3, G, N, ldw = _check_weight("fp8_matmul", w, w_scale, K, dev)
-    _check_offsets("fp8_matmul", offsets, G, dev)
     if out is None:
-        out = torch.empty((M, N), device=dev, dtype=out_dtype)
-    elif out.shape != (M, N) or (out.stride(1) != 1 and N > 1) or out.device != dev:
-        raise ValueError("fp8_matmul: out must be (M, N) on the rows' device with unit column stride")
-    L = nat.lib()
-    with nat.on_device(dev):
-        rc = L.rwkv_fp8_gemm(nat.ptr(a), nat.row_stride(a), nat.ptr(a_scale), nat.ptr(w3), ldw, w3.stride(0), nat.ptr(s3),
-                             nat.ptr(offsets), nat.ptr(out), nat.row_stride(out), M, N, K, G, int(relu_sq),
-                             nat.dtype_code(out), nat.stream_ptr(dev))
-    nat.check(rc, "rwkv_fp8_gemm")
+        out = torch.empty((a.shape[0], w.shape[-2]), device=a.device, dtype=out_dtype)
+    _gemm("fp8_matmul", a, a_scale, w, w_scale, offsets, out, None, int(relu_sq), nat.dtype_code(out))
     return out
 
 
+def fp8_matmul_relu_sq_quantized(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                                 offsets: torch.Tensor | None = None):
+    """relu(a @ w^T)^2 quantised like :func:`quantize_fp8_rows` inside the product's kernel (the hidden
+    rows of a squared-ReLU layer): returns (q (M, N) e4m3, scale (M, ceil(N / 128)))."""
+    M, N, dev = a.shape[0], w.shape[-2], a.device
+    q = _empty_e4m3(M, N, dev)
+    scale = torch.empty((_blocks(N), M), device=dev, dtype=torch.float32)
+    _gemm("fp8_matmul_relu_sq_quantized", a, a_scale, w, w_scale, offsets, q, scale, 2, 0)
+    return q, scale.t()
+
+
 def _linear(x2d, w, w_scale):
-    q, s = quantize_fp8_rows(x2d)
-    return fp8_matmul(q, s, w, w_scale, out_dtype=x2d.dtype)
+    """x2d has unit column stride; the weight is checked here, the rest by the library."""
+    M, K = x2d.shape
+    dev = x2d.device
+    if w.dtype != E4M3 or w.device != dev or w_scale.dtype != torch.float32 or w_scale.device != dev \
+            or w_scale.shape != (_blocks(w.shape[0]), _blocks(K)) or (K > 1 and w.stride(1) != 1):
+        raise ValueError(f"fp8_linear: the weight must be e4m3 (N, {K}) with unit column stride and fp32 scales "
+                         "(ceil(N / 128), ceil(K / 128)) on x's device")
+    N = w.shape[0]
+    code = nat.dtype_code(x2d)
+    out = torch.empty((M, N), device=dev, dtype=x2d.dtype)
+    L = nat.lib()
+    nws = L.rwkv_fp8_linear_workspace_size(M, K)
+    ws = torch.empty(nws, device=dev, dtype=torch.uint8)
+    with nat.on_device(dev):
+        rc = L.rwkv_fp8_linear(x2d.data_ptr(), nat.row_stride(x2d), w.data_ptr(), nat.row_stride(w),
+                               w_scale.contiguous().data_ptr(), out.data_ptr(), N, ws.data_ptr(), nws, M, N, K, code,
+                               nat.stream_ptr(dev))
+    nat.check(rc, "rwkv_fp8_linear")
+    return out
 
 
 class _Linear(torch.autograd.Function):
@@ -163,7 +195,7 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _linear(dy, *ctx.saved_tensors), None, None, None, None
+        return _linear(nat.rows_2d(dy), *ctx.saved_tensors), None, None, None, None
 
 
 def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, w_t: torch.Tensor | None = None,
@@ -173,15 +205,15 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, w_t: tor
     The weight is frozen.  For an x that requires grad, pass the transposed layout
     (:func:`transpose_fp8_weight`, kept beside the weight): dx = q(dy) @ w runs on the same kernels,
     with dy quantised like x."""
-    if w.dim() != 2:
-        raise ValueError("fp8_linear: w must be (N, K)")
-    if x.shape[-1] != w.shape[1]:
-        raise ValueError(f"fp8_linear: x has {x.shape[-1]} columns, the weight {w.shape[1]}")
+    if w.dim() != 2 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"fp8_linear: x {tuple(x.shape)} and w {tuple(w.shape)} do not fit (w is (N, K))")
     x2 = nat.rows_2d(x)
     if x.requires_grad and torch.is_grad_enabled():
         if w_t is None or w_scale_t is None:
             raise RuntimeError("fp8_linear: an input that requires grad needs the transposed weight "
                                "(transpose_fp8_weight) for the gradient")
+        if w_t.shape != (w.shape[1], w.shape[0]):
+            raise ValueError("fp8_linear: w_t must be (K, N)")
         y = _Linear.apply(x2, w, w_scale, w_t, w_scale_t)
     else:
         y = _linear(x2, w, w_scale)
@@ -196,7 +228,24 @@ def fp8_experts(rows: torch.Tensor, key: torch.Tensor, key_scale: torch.Tensor, 
     value (E, C, D) e4m3 with their scales.  Rows outside every expert are undefined.  Forward only."""
     if torch.is_grad_enabled() and rows.requires_grad:
         raise RuntimeError("fp8_experts: forward only; call it under torch.no_grad() or on rows without gradient")
-    q, s = quantize_fp8_rows(rows)
-    h = fp8_matmul(q, s, key, key_scale, offsets, relu_sq=True, out_dtype=torch.float32)
-    q, s = quantize_fp8_rows(h)
-    return fp8_matmul(q, s, value, value_scale, offsets, out_dtype=rows.dtype)
+    if rows.dim() != 2 or key.dim() != 3 or value.dim() != 3 or value.shape != (key.shape[0], key.shape[2], key.shape[1]) \
+            or key.shape[2] != rows.shape[1]:
+        raise ValueError(f"fp8_experts: rows {tuple(rows.shape)}, key {tuple(key.shape)} and value {tuple(value.shape)} "
+                         "do not fit (key (E, D, C), value (E, C, D))")
+    code = nat.dtype_code(rows)
+    x = nat.rows_2d(rows)
+    M, C = x.shape
+    dev = x.device
+    key, key_scale, E, D, ldk = _check_weight("fp8_experts", key, key_scale, C, dev)
+    value, value_scale, _, _, ldv = _check_weight("fp8_experts", value, value_scale, D, dev)
+    _check_offsets("fp8_experts", offsets, E, dev)
+    out = torch.empty((M, C), device=dev, dtype=x.dtype)
+    L = nat.lib()
+    nws = L.rwkv_fp8_experts_workspace_size(M, C, D, E)
+    ws = torch.empty(nws, device=dev, dtype=torch.uint8)
+    with nat.on_device(dev):
+        rc = L.rwkv_fp8_experts(x.data_ptr(), nat.row_stride(x), key.data_ptr(), ldk, key.stride(0), key_scale.data_ptr(),
+                                value.data_ptr(), ldv, value.stride(0), value_scale.data_ptr(), nat.ptr(offsets),
+                                out.data_ptr(), C, ws.data_ptr(), nws, M, C, D, E, code, nat.stream_ptr(dev))
+    nat.check(rc, "rwkv_fp8_experts")
+    return out
