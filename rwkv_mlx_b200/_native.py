@@ -175,6 +175,8 @@ def ptr(t: torch.Tensor | None):
 
 
 def stream_ptr(device=None):
+    if device is not None and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)  # the same handle, without a Stream object
     return torch.cuda.current_stream(device).cuda_stream
 
 

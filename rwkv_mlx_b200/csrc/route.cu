@@ -36,11 +36,11 @@ struct Args {
     float scale;
 };
 
-// Unsigned order of a float: NaN highest, -0 equal to +0.  Never 0 (the excluded key).
+// Unsigned order of a float that an addition has produced (so NaN is the canonical positive one,
+// which orders above +inf, and there is no -0).  Never 0, the key of what cannot be chosen.
 __device__ __forceinline__ uint32_t okey(float f) {
-    if (f != f) return 0xffffffffu;
-    const uint32_t u = __float_as_uint(f + 0.f);
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    const uint32_t u = __float_as_uint(f);
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float sigmoidf(float x) { return __frcp_rn(1.f + expf(-x)); }
 
@@ -81,13 +81,26 @@ __device__ __forceinline__ void load_row(const T* row, int e0, int E, bool vec, 
 
 // Two largest of (a1 >= a2) and (b1 >= b2) as ordered keys.
 __device__ __forceinline__ void merge2(uint32_t& a1, uint32_t& a2, uint32_t b1, uint32_t b2) {
-    const uint32_t lo = min(a1, b1);
+    a2 = max(min(a1, b1), max(a2, b2));
     a1 = max(a1, b1);
-    a2 = max(lo, max(a2, b2));
 }
 __device__ __forceinline__ float unkey(uint32_t u) {
-    if (u == 0xffffffffu) return __int_as_float(0x7fc00000);
-    return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+    return __uint_as_float(u ^ ((uint32_t)((int)~u >> 31) | 0x80000000u));
+}
+
+// The lane's two largest keys outside `gone` and their positions (ties: the lower position first).
+template <int EPL>
+__device__ __forceinline__ void local2(const uint32_t (&key)[EPL], uint32_t gone, uint32_t& k1, int& i1, uint32_t& k2, int& i2) {
+    k1 = k2 = 0u, i1 = i2 = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; i++) {
+        const uint32_t k = (gone >> i) & 1u ? 0u : key[i];
+        const bool p1 = k > k1, p2 = k > k2;
+        i2 = p1 ? i1 : (p2 ? i : i2);
+        i1 = p1 ? i : i1;
+        k2 = max(k2, min(k1, k));
+        k1 = max(k1, k);
+    }
 }
 
 template <typename T, int EPL>
@@ -95,7 +108,8 @@ __global__ void __launch_bounds__(NT) route_kernel(const Args p) {
     extern __shared__ uint32_t smem_route[];
     uint32_t* hist = smem_route;                                        // E counters (counts only)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E;
-    uint32_t* wkeys = smem_route + (p.counts ? E : 0) + warp * E;       // this warp's keys (odd group sizes only)
+    int* sel = reinterpret_cast<int*>(smem_route + (p.counts ? E : 0)) + warp * MAXK;   // this warp's choices
+    uint32_t* wkeys = smem_route + (p.counts ? E : 0) + NW * MAXK + warp * E;  // its keys (odd group sizes only)
     if (p.counts) {
         for (int e = threadIdx.x; e < E; e += NT) hist[e] = 0;
         __syncthreads();
@@ -103,16 +117,21 @@ __global__ void __launch_bounds__(NT) route_kernel(const Args p) {
     const int e0 = lane * EPL, per = E / p.groups;
     const int lanes_per = per / EPL;  // lanes of a group, when the layout is aligned
     const bool by_lanes = per % EPL == 0 && (lanes_per & (lanes_per - 1)) == 0;
+    const bool by_logit = !p.sigmoid && !p.bias && !(p.groups > 1 && p.top2);
     float b[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; i++) b[i] = p.bias && e0 + i < E ? p.bias[e0 + i] : 0.f;
 
-    for (int t = blockIdx.x * NW + warp; t < p.n; t += gridDim.x * NW) {
+    float next[EPL];  // the next token's logits load during this token's selection
+    int t = blockIdx.x * NW + warp;
+    if (t < p.n) load_row<T, EPL>(reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld, e0, E, p.vec, next);
+    for (; t < p.n; t += gridDim.x * NW) {
         const T* row = reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld;
         float l[EPL];
-        load_row<T, EPL>(row, e0, E, p.vec, l);
+#pragma unroll
+        for (int i = 0; i < EPL; i++) l[i] = next[i];
+        if (t + (int)gridDim.x * NW < p.n) load_row<T, EPL>(row + (long long)gridDim.x * NW * p.ld, e0, E, p.vec, next);
         float m = 0.f, z = 0.f;  // softmax: row maximum (0 for a row of -inf) and sum
-        const bool by_logit = !p.sigmoid && !p.bias && !(p.groups > 1 && p.top2);
         if (!p.sigmoid && (!by_logit || !p.renorm)) {
             m = -INFINITY;
 #pragma unroll
@@ -129,15 +148,16 @@ __global__ void __launch_bounds__(NT) route_kernel(const Args p) {
             float f = l[i];
             if (p.sigmoid) f = sigmoidf(f);
             else if (!by_logit) f = z == 0.f ? 0.f : expf(f - m) / z;
-            if (p.bias) f += b[i];
-            key[i] = e0 + i < E ? okey(f) : 0u;
+            key[i] = e0 + i < E ? okey(f + b[i]) : 0u;
         }
+        uint32_t k1, k2;  // the lane's two best keys: most tokens take at most two experts from a lane
+        int i1, i2;
+        local2<EPL>(key, 0u, k1, i1, k2, i2);
         if (p.groups > 1) {
-            uint32_t g1 = 0, g2 = 0;  // two largest keys of this lane's group
-            int mine;                 // the group that this lane ranks
+            uint32_t g1 = 0, g2 = 0;  // two largest keys of the group that this lane ranks
+            int mine;
             if (by_lanes) {
-#pragma unroll
-                for (int i = 0; i < EPL; i++) merge2(g1, g2, key[i], 0u);
+                g1 = k1, g2 = k2;
                 for (int o = 1; o < lanes_per; o <<= 1)
                     merge2(g1, g2, __shfl_xor_sync(0xffffffffu, g1, o), __shfl_xor_sync(0xffffffffu, g2, o));
                 mine = lane / lanes_per;
@@ -151,46 +171,41 @@ __global__ void __launch_bounds__(NT) route_kernel(const Args p) {
                     for (int i = 0; i < per; i++) merge2(g1, g2, wkeys[lane * per + i], 0u);
                 __syncwarp();
             }
-            uint32_t gs = g1;
-            if (p.top2 && per > 1) gs = okey(unkey(g1) + unkey(g2));
+            const uint32_t gs = p.top2 && per > 1 ? okey(unkey(g1) + unkey(g2)) : g1;
             int rank = 0;
-            for (int g = 0; g < p.groups; g++) {
-                const uint32_t o = __shfl_sync(0xffffffffu, gs, by_lanes ? g * lanes_per : g);
-                rank += (o > gs || (o == gs && g < mine)) ? 1 : 0;
-            }
-            const uint32_t stay = __ballot_sync(0xffffffffu, rank < p.keep && mine < p.groups);
-            if (by_lanes) {
-                if (!((stay >> lane) & 1u)) {
-#pragma unroll
-                    for (int i = 0; i < EPL; i++) key[i] = 0u;
+            if (by_lanes) {  // the group's lanes share the comparisons
+                for (int g = lane & (lanes_per - 1); g < p.groups + (lane & (lanes_per - 1)); g += lanes_per) {
+                    const uint32_t o = __shfl_sync(0xffffffffu, gs, g * lanes_per);
+                    if (g < p.groups) rank += (o > gs || (o == gs && g < mine)) ? 1 : 0;
                 }
+                for (int o = 1; o < lanes_per; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+                if (rank >= p.keep || mine >= p.groups) k1 = k2 = 0u;
             } else {
+                for (int g = 0; g < p.groups; g++) {
+                    const uint32_t o = __shfl_sync(0xffffffffu, gs, g);
+                    rank += (o > gs || (o == gs && g < mine)) ? 1 : 0;
+                }
+                const uint32_t stay = __ballot_sync(0xffffffffu, rank < p.keep && mine < p.groups);
 #pragma unroll
                 for (int i = 0; i < EPL; i++)
                     if (e0 + i < E && !((stay >> ((e0 + i) / per)) & 1u)) key[i] = 0u;
+                local2<EPL>(key, 0u, k1, i1, k2, i2);
             }
         }
-        // top-k: lane j ends up with the j-th choice
-        uint32_t best = 0;
-        int bi = 0, choice = 0;
-#pragma unroll
-        for (int i = 0; i < EPL; i++)
-            if (key[i] > best) best = key[i], bi = i;
+        // top-k: the j-th choice goes to sel[j]
+        uint32_t gone = 0;
         for (int j = 0; j < p.k; j++) {
-            const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-            const int src = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
-            const int e = __shfl_sync(0xffffffffu, e0 + bi, src);
-            if (lane == j) choice = e;
-            if (lane == src) {
-                best = 0;
-                const int gone = bi;
-#pragma unroll
-                for (int i = 0; i < EPL; i++) {
-                    if (i == gone) key[i] = 0u;
-                    if (key[i] > best) best = key[i], bi = i;
-                }
+            const uint32_t top = __reduce_max_sync(0xffffffffu, k1);
+            if (lane == __ffs(__ballot_sync(0xffffffffu, k1 == top)) - 1) {
+                sel[j] = e0 + i1;
+                gone |= 1u << i1;
+                if (EPL > 2 && k2 == 0u) local2<EPL>(key, gone, k1, i1, k2, i2);
+                else k1 = k2, i1 = i2, k2 = 0u;
             }
         }
+        __syncwarp();
+        const int choice = sel[lane];
+        __syncwarp();
         const bool on = lane < p.k;
         float s = 0.f;
         if (p.sigmoid) {
@@ -316,7 +331,7 @@ template <typename T, int EPL>
 static void launch_fwd(const Args& p, int grid, cudaStream_t st) {
     const int per = p.E / p.groups, lp = per / EPL;
     const bool by_lanes = per % EPL == 0 && (lp & (lp - 1)) == 0;
-    const size_t smem = sizeof(uint32_t) * ((p.counts ? p.E : 0) + (p.groups > 1 && !by_lanes ? NW * p.E : 0));
+    const size_t smem = sizeof(uint32_t) * (NW * MAXK + (p.counts ? p.E : 0) + (p.groups > 1 && !by_lanes ? NW * p.E : 0));
     route_kernel<T, EPL><<<grid, NT, smem, st>>>(p);
 }
 template <typename T, int EPL>

@@ -40,10 +40,13 @@ class _Route(torch.autograd.Function):
         ctx.save_for_backward(logits, inds, weights)
         ctx.opts = (sigmoid, renormalize, scale)
         ctx.mark_non_differentiable(inds, *([] if counts is None else [counts]))
+        ctx.set_materialize_grads(False)  # no zero tensors for the integer outputs
         return inds, weights, counts
 
     @staticmethod
     def backward(ctx, _dinds, dweights, _dcounts=None):
+        if dweights is None:
+            return (None,) * 10
         logits, inds, weights = ctx.saved_tensors
         sigmoid, renormalize, scale = ctx.opts
         n, E = logits.shape
