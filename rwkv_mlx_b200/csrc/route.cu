@@ -44,6 +44,26 @@ __device__ __forceinline__ uint32_t okey(float f) {
 }
 __device__ __forceinline__ float sigmoidf(float x) { return __frcp_rn(1.f + expf(-x)); }
 
+// sigmoidf of a lane's logits.  For 1 <= d < 2^100 one Newton step from rcp.approx (within an ulp)
+// gives the correctly rounded reciprocal (Markstein 1990; checked against __frcp_rn for every such
+// float), without a branch an element; rows with larger d take __frcp_rn.
+template <int EPL>
+__device__ __forceinline__ void sigmoid_row(const float (&l)[EPL], float (&s)[EPL]) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPL; i++) {
+        const float d = 1.f + expf(-l[i]);
+        float y;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d));
+        s[i] = fmaf(y, fmaf(-d, y, 1.f), y);
+        top = fmaxf(top, d);
+    }
+    if (top >= 0x1p100f) {
+#pragma unroll
+        for (int i = 0; i < EPL; i++) s[i] = sigmoidf(l[i]);
+    }
+}
+
 __device__ __forceinline__ float wmax(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -103,8 +123,11 @@ __device__ __forceinline__ void local2(const uint32_t (&key)[EPL], uint32_t gone
     }
 }
 
-template <typename T, int EPL>
-__global__ void __launch_bounds__(NT) route_kernel(const Args p) {
+// Groups: none, runs of lanes (their size a power of two times EPL), or any equal runs.
+enum Groups { ONE = 0, LANES = 1, ANY = 2 };
+
+template <typename T, int EPL, bool SIG, int GROUPS>
+__global__ void __launch_bounds__(NT, EPL <= 8 ? 4 : 2) route_kernel(const Args p) {
     extern __shared__ uint32_t smem_route[];
     uint32_t* hist = smem_route;                                        // E counters (counts only)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E;
@@ -115,9 +138,8 @@ __global__ void __launch_bounds__(NT) route_kernel(const Args p) {
         __syncthreads();
     }
     const int e0 = lane * EPL, per = E / p.groups;
-    const int lanes_per = per / EPL;  // lanes of a group, when the layout is aligned
-    const bool by_lanes = per % EPL == 0 && (lanes_per & (lanes_per - 1)) == 0;
-    const bool by_logit = !p.sigmoid && !p.bias && !(p.groups > 1 && p.top2);
+    const int lanes_per = per / EPL;  // LANES: lanes of a group
+    const bool by_logit = !SIG && !p.bias && !(GROUPS != ONE && p.top2);
     float b[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; i++) b[i] = p.bias && e0 + i < E ? p.bias[e0 + i] : 0.f;
@@ -132,7 +154,7 @@ __global__ void __launch_bounds__(NT) route_kernel(const Args p) {
         for (int i = 0; i < EPL; i++) l[i] = next[i];
         if (t + (int)gridDim.x * NW < p.n) load_row<T, EPL>(row + (long long)gridDim.x * NW * p.ld, e0, E, p.vec, next);
         float m = 0.f, z = 0.f;  // softmax: row maximum (0 for a row of -inf) and sum
-        if (!p.sigmoid && (!by_logit || !p.renorm)) {
+        if (!SIG && (!by_logit || !p.renorm)) {
             m = -INFINITY;
 #pragma unroll
             for (int i = 0; i < EPL; i++) m = (l[i] > m || l[i] != l[i]) ? l[i] : m;
@@ -143,20 +165,22 @@ __global__ void __launch_bounds__(NT) route_kernel(const Args p) {
             z = wsum(z);
         }
         uint32_t key[EPL];
+        float f[EPL];
+        if (SIG) {
+            sigmoid_row<EPL>(l, f);
+        } else {
 #pragma unroll
-        for (int i = 0; i < EPL; i++) {
-            float f = l[i];
-            if (p.sigmoid) f = sigmoidf(f);
-            else if (!by_logit) f = z == 0.f ? 0.f : expf(f - m) / z;
-            key[i] = e0 + i < E ? okey(f + b[i]) : 0u;
+            for (int i = 0; i < EPL; i++) f[i] = by_logit ? l[i] : (z == 0.f ? 0.f : expf(l[i] - m) / z);
         }
+#pragma unroll
+        for (int i = 0; i < EPL; i++) key[i] = e0 + i < E ? okey(f[i] + b[i]) : 0u;
         uint32_t k1, k2;  // the lane's two best keys: most tokens take at most two experts from a lane
         int i1, i2;
         local2<EPL>(key, 0u, k1, i1, k2, i2);
-        if (p.groups > 1) {
+        if (GROUPS != ONE) {
             uint32_t g1 = 0, g2 = 0;  // two largest keys of the group that this lane ranks
             int mine;
-            if (by_lanes) {
+            if (GROUPS == LANES) {
                 g1 = k1, g2 = k2;
                 for (int o = 1; o < lanes_per; o <<= 1)
                     merge2(g1, g2, __shfl_xor_sync(0xffffffffu, g1, o), __shfl_xor_sync(0xffffffffu, g2, o));
@@ -173,7 +197,7 @@ __global__ void __launch_bounds__(NT) route_kernel(const Args p) {
             }
             const uint32_t gs = p.top2 && per > 1 ? okey(unkey(g1) + unkey(g2)) : g1;
             int rank = 0;
-            if (by_lanes) {  // the group's lanes share the comparisons
+            if (GROUPS == LANES) {  // the group's lanes share the comparisons
                 for (int g = lane & (lanes_per - 1); g < p.groups + (lane & (lanes_per - 1)); g += lanes_per) {
                     const uint32_t o = __shfl_sync(0xffffffffu, gs, g * lanes_per);
                     if (g < p.groups) rank += (o > gs || (o == gs && g < mine)) ? 1 : 0;
@@ -196,19 +220,19 @@ __global__ void __launch_bounds__(NT) route_kernel(const Args p) {
         uint32_t gone = 0;
         for (int j = 0; j < p.k; j++) {
             const uint32_t top = __reduce_max_sync(0xffffffffu, k1);
-            if (lane == __ffs(__ballot_sync(0xffffffffu, k1 == top)) - 1) {
-                sel[j] = e0 + i1;
-                gone |= 1u << i1;
-                if (EPL > 2 && k2 == 0u) local2<EPL>(key, gone, k1, i1, k2, i2);
-                else k1 = k2, i1 = i2, k2 = 0u;
-            }
+            const bool win = lane == __ffs(__ballot_sync(0xffffffffu, k1 == top)) - 1;
+            if (win) sel[j] = e0 + i1;
+            gone |= win ? 1u << i1 : 0u;
+            const bool again = EPL > 2 && win && k2 == 0u;
+            k1 = win ? k2 : k1, i1 = win ? i2 : i1, k2 = win ? 0u : k2;
+            if (again) local2<EPL>(key, gone, k1, i1, k2, i2);
         }
         __syncwarp();
         const int choice = sel[lane];
         __syncwarp();
         const bool on = lane < p.k;
         float s = 0.f;
-        if (p.sigmoid) {
+        if (SIG) {
             if (on) s = sigmoidf(to_f32(row[choice]));
         } else {
             const float lj = on ? to_f32(row[choice]) : -INFINITY;
@@ -330,9 +354,15 @@ static int grid_for(int n, int per_sm) {
 template <typename T, int EPL>
 static void launch_fwd(const Args& p, int grid, cudaStream_t st) {
     const int per = p.E / p.groups, lp = per / EPL;
-    const bool by_lanes = per % EPL == 0 && (lp & (lp - 1)) == 0;
-    const size_t smem = sizeof(uint32_t) * (NW * MAXK + (p.counts ? p.E : 0) + (p.groups > 1 && !by_lanes ? NW * p.E : 0));
-    route_kernel<T, EPL><<<grid, NT, smem, st>>>(p);
+    const int mode = p.groups == 1 ? ONE : per % EPL == 0 && (lp & (lp - 1)) == 0 ? LANES : ANY;
+    const size_t smem = sizeof(uint32_t) * (NW * MAXK + (p.counts ? p.E : 0) + (mode == ANY ? NW * p.E : 0));
+    auto kern = p.sigmoid ? (mode == ONE     ? route_kernel<T, EPL, true, ONE>
+                             : mode == LANES ? route_kernel<T, EPL, true, LANES>
+                                             : route_kernel<T, EPL, true, ANY>)
+                          : (mode == ONE     ? route_kernel<T, EPL, false, ONE>
+                             : mode == LANES ? route_kernel<T, EPL, false, LANES>
+                                             : route_kernel<T, EPL, false, ANY>);
+    kern<<<grid, NT, smem, st>>>(p);
 }
 template <typename T, int EPL>
 static void launch_bwd(const BwdArgs& p, int grid, cudaStream_t st) {
