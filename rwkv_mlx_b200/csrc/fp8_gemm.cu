@@ -119,6 +119,7 @@ int gemm_stream(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st) {
 }
 
 static int g_gemm_impl = 0;
+extern int g_tc_impl;
 
 // Few rows: the weights are read once at most for every 32 rows of a group, and 16-row tiles
 // of W keep the SMs busy where 128 x 128 output tiles would not.
@@ -239,7 +240,8 @@ extern "C" int rwkv_fp8_experts(const void* x, long long ldx, const void* key, l
 }
 
 extern "C" int rwkv_fp8_set_gemm_impl(int impl) {
-    if (impl < 0 || impl > 2) return RWKV_ERR_ARG;
+    if (impl < 0 || impl > 3) return RWKV_ERR_ARG;
     fp8::g_gemm_impl = impl;
+    fp8::g_tc_impl = impl;
     return RWKV_OK;
 }

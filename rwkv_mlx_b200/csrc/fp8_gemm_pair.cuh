@@ -1,0 +1,383 @@
+// e4m3 products by CTA pairs (included by fp8_gemm_tc.cu): the method of that file on tiles of
+// 256 x 256, which one pair of SMs computes with cta_group::2 MMAs.  Each CTA loads 128 rows of A
+// and 128 rows of W a stage (32 KB instead of the 48 KB that a 128 x 256 tile needs for half the
+// products) and keeps 128 rows of the result.
+//
+// A K block's product is issued as two MMA groups of 256 x 128, so that tensor memory holds four
+// accumulators of 128 columns: columns h * 128 .. + 127 of the tile belong to the drain warps of
+// half h, and an accumulator is refilled two blocks after it was handed over.
+//   warp 8 lane 0   producer: A (128 rows) and twice W (64 rows of each column half) by TMA,
+//                   signalled on the CTA's own "full" barrier;
+//   warp 9 lane 0   CTA 0: MMA issuer for the pair; CTA 1: forwards its "full" barriers to CTA 0
+//                   (a load here signals only its own CTA, so that each CTA can drain its own
+//                   copies when it has to give up);
+//   warps 0-7       drain and epilogue.  A warp lays its 32 x 128 outputs out in shared memory in
+//                   the tensor map's swizzle and hands them to TMA, which stores them while the
+//                   next tile is being computed; rows of another group's are guarded one by one.
+// Commits arrive in both CTAs (multicast of the arrival, not of data).
+#pragma once
+#include "fp8_tc.cuh"
+
+namespace rwkv {
+namespace fp8 {
+
+constexpr int PM = 256, PN = 256, PNS = 5;
+constexpr int PA_BYTES = BM * BLK, PW_BYTES = 64 * BLK, PSTAGE = PA_BYTES + 2 * PW_BYTES;
+constexpr int POUT = 8192;  // output staging of a drain warp
+
+struct PairCtrl {
+    unsigned long long full[PNS], empty[PNS], peer_full[PNS], acc_full[4], acc_empty[4], drain;
+    uint32_t tmem_base;
+    int abort;
+    Groups groups;
+};
+constexpr int PAIR_SMEM = PNS * PSTAGE + NDRAIN / 32 * POUT + 3072;
+static_assert(sizeof(PairCtrl) <= 3072 && PAIR_SMEM <= 227 * 1024, "shared memory");
+
+__device__ __forceinline__ void umma8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p; }" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// Arrives on this barrier in both CTAs of the pair when the MMAs issued so far have completed.
+__device__ __forceinline__ void commit_pair(unsigned long long* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            ck::smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void arrive_cta0(unsigned long long* bar) {
+    asm volatile(
+        "{ .reg .b32 ra; mapa.shared::cluster.u32 ra, %0, 0; "
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra]; }" ::"r"(ck::smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// wait_f for a barrier on which the other CTA arrives.
+__device__ __forceinline__ bool wait_c(unsigned long long* b, uint32_t parity, volatile int* abort) {
+    const uint32_t a = ck::smem_u32(b);
+    long long t0 = 0;
+    while (true) {
+        uint32_t ok;
+        asm volatile(
+            "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+            : "=r"(ok)
+            : "r"(a), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (*abort) return false;
+        if (t0 == 0) t0 = clock64();
+        if (clock64() - t0 > ck::WAIT_CYCLES) {
+            *abort = 1;
+            atomicOr(&g_device_error_fp8, 1);
+            return false;
+        }
+    }
+}
+
+}  // namespace fp8
+
+template <int EPI, typename TO>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp8::NTH, 1)
+    fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mw,
+                         const __grid_constant__ CUtensorMap mo, const fp8::GemmArgs p, const int tma_out) {
+    using namespace fp8;
+    constexpr uint32_t IDESC = idesc_e4m3(PM, 128);
+
+    extern __shared__ __align__(1024) unsigned char smem_pair[];
+    unsigned char* ring = smem_pair;                       // stage: A box, W box of half 0, W box of half 1
+    unsigned char* stage_out = ring + PNS * PSTAGE;        // 8 KB per drain warp
+    PairCtrl& cs = *reinterpret_cast<PairCtrl*>(stage_out + NDRAIN / 32 * POUT);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = blockIdx.x & 1, pair0 = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int nk = (p.K + BLK - 1) / BLK, ntn = (p.N + PN - 1) / PN;
+
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(ck::smem_u32(&cs.tmem_base))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    if (tid == NDRAIN) {
+        for (int i = 0; i < PNS; i++) {
+            ck::mbar_init(&cs.full[i], 1), ck::mbar_init(&cs.empty[i], 1), ck::mbar_init(&cs.peer_full[i], 1);
+        }
+        for (int i = 0; i < 4; i++) ck::mbar_init(&cs.acc_full[i], 1), ck::mbar_init(&cs.acc_empty[i], 8);
+        ck::mbar_init(&cs.drain, 1);
+        // the swizzle needs the ring on a 1024-byte boundary; nothing runs if it is not there
+        cs.abort = c_force_wait_timeout_fp8 || (ck::smem_u32(ring) & 1023) ? 1 : 0;
+        if (cs.abort) atomicOr(&g_device_error_fp8, 2);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    load_offsets(cs.groups, p, tid);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) scan_units(cs.groups, p.G, PM, ntn, lane);
+    __syncthreads();
+    cluster_sync();  // the other CTA's barriers exist and its tensor memory is allocated
+    const uint32_t tmem = cs.tmem_base;
+    const int nunits = cs.groups.unit[p.G];
+
+    if (warp >= NDRAIN / 32) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_ISSUE));
+        if (warp == NDRAIN / 32) {
+            // ===================== producer =====================
+            if (lane == 0) {
+                int it = 0, s = 0;
+                uint32_t ph = 0;
+                bool bad = false;
+                for (int u = pair0; u < nunits && !bad && !*(volatile int*)&cs.abort; u += npairs) {
+                    const Unit un = unit_of(cs.groups, p.G, PM, ntn, u);
+                    const int row = un.row0 + rank * BM, n0 = un.nt * PN + rank * 64;
+                    for (int kb = 0; kb < nk; kb++, it++) {
+                        if (it >= PNS && !wait_f(&cs.empty[s], ph ^ 1, &cs.abort)) {
+                            bad = true;
+                            break;
+                        }
+                        unsigned char* st = ring + s * PSTAGE;
+                        expect_tx(&cs.full[s], PSTAGE);
+                        tma_load_2d(st, &ma, kb * BLK, row, &cs.full[s]);
+                        tma_load_3d(st + PA_BYTES, &mw, kb * BLK, n0, un.g, &cs.full[s]);
+                        tma_load_3d(st + PA_BYTES + PW_BYTES, &mw, kb * BLK, n0 + 128, un.g, &cs.full[s]);
+                        if (++s == PNS) s = 0, ph ^= 1;
+                    }
+                }
+                // shared memory stays allocated until the last copies have landed
+                for (int i = (it > PNS ? it - PNS : 0); i < it; i++)
+                    ck::mbar_drain(&cs.full[i % PNS], (i / PNS) & 1, &g_device_error_fp8);
+            }
+            __syncwarp();
+        } else if (warp == NDRAIN / 32 + 1 && lane == 0) {
+            int it = 0, s = 0;
+            uint32_t ph = 0;
+            bool bad = false;
+            if (rank == 1) {
+                // ===================== forwarder =====================
+                for (int u = pair0; u < nunits && !bad && !*(volatile int*)&cs.abort; u += npairs)
+                    for (int kb = 0; kb < nk; kb++) {
+                        if (!wait_f(&cs.full[s], ph, &cs.abort)) {
+                            bad = true;
+                            break;
+                        }
+                        arrive_cta0(&cs.peer_full[s]);
+                        if (++s == PNS) s = 0, ph ^= 1;
+                    }
+            } else {
+                // ===================== MMA issuer =====================
+                const uint64_t desc_a = desc_sw128(ck::smem_u32(ring), 16, 1024);
+                for (int u = pair0; u < nunits && !bad && !*(volatile int*)&cs.abort; u += npairs)
+                    for (int kb = 0; kb < nk && !bad; kb++, it++) {
+                        if (!wait_f(&cs.full[s], ph, &cs.abort) || !wait_c(&cs.peer_full[s], ph, &cs.abort)) {
+                            bad = true;
+                            break;
+                        }
+                        const uint64_t da = desc_a + s * (PSTAGE >> 4);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int b = (it & 1) * 2 + h;  // accumulator; refilled every second block
+                            if (it >= 2 && !wait_c(&cs.acc_empty[b], ((it >> 1) + 1) & 1, &cs.abort)) {
+                                bad = true;
+                                break;
+                            }
+                            tc_fence_after();
+#pragma unroll
+                            for (int kk = 0; kk < BLK / 32; kk++)
+                                umma8_pair(tmem + b * 128, da + kk * 2, da + ((PA_BYTES + h * PW_BYTES) >> 4) + kk * 2,
+                                           IDESC, kk > 0 ? 1u : 0u);
+                            commit_pair(&cs.acc_full[b]);
+                        }
+                        if (bad) break;
+                        commit_pair(&cs.empty[s]);
+                        if (++s == PNS) s = 0, ph ^= 1;
+                    }
+                // wait for this thread's own MMAs before either CTA's memory is freed
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                                 ck::smem_u32(&cs.drain))
+                             : "memory");
+                ck::mbar_drain(&cs.drain, 0, &g_device_error_fp8);
+            }
+        }
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_DRAIN));
+        // ===================== drain and epilogue =====================
+        const int ew = warp & 3, half = warp >> 2;
+        const int rl = 32 * ew + lane;  // row of the CTA's half tile = TMEM lane
+        const uint32_t tl = tmem + ((uint32_t)(32 * ew) << 16) + half * 128;
+        const int nbn = (p.N + BLK - 1) / BLK;
+        unsigned char* buf = stage_out + warp * POUT;
+        bool ab = *(volatile int*)&cs.abort != 0;
+        int it = 0;
+        // scales are loaded PF blocks at a time, one group of blocks ahead (fp8_gemm_tc_kernel)
+        constexpr int PF = 2;
+        float sa[PF], sb[PF];
+        const float *sap = nullptr, *sbp = nullptr;
+        auto aim = [&](const Unit& un) {
+            const int row = un.row0 + rank * BM + rl, nb = min(un.nt * 2 + half, nbn - 1);
+            sap = row < un.rend ? p.as + row : nullptr;
+            sbp = p.ws + ((long long)un.g * nbn + nb) * nk;
+        };
+        auto fetch = [&](int kb0) {
+#pragma unroll
+            for (int i = 0; i < PF; i++) {
+                const bool on = kb0 + i < nk;
+                sa[i] = on && sap ? __ldg(sap + (long long)(kb0 + i) * p.M) : 0.f;
+                sb[i] = on ? __ldg(sbp + kb0 + i) : 0.f;
+            }
+        };
+        if (pair0 < nunits) {
+            aim(unit_of(cs.groups, p.G, PM, ntn, pair0));
+            fetch(0);
+        }
+        for (int u = pair0; u < nunits; u += npairs) {
+            const Unit un = unit_of(cs.groups, p.G, PM, ntn, u);
+            const int row0 = un.row0 + rank * BM + 32 * ew, n0 = un.nt * PN + half * 128;
+            float acc[BLK];
+#pragma unroll
+            for (int c = 0; c < BLK; c++) acc[c] = 0.f;
+            for (int kb0 = 0; kb0 < nk && !ab; kb0 += PF) {
+                float s[PF];
+#pragma unroll
+                for (int i = 0; i < PF; i++) s[i] = sa[i] * sb[i];
+                if (kb0 + PF < nk) {
+                    fetch(kb0 + PF);
+                } else if (u + npairs < nunits) {
+                    aim(unit_of(cs.groups, p.G, PM, ntn, u + npairs));
+                    fetch(0);
+                }
+#pragma unroll
+                for (int i = 0; i < PF; i++) {
+                    if (kb0 + i >= nk || ab) break;
+                    const int b = (it & 1) * 2 + half;
+                    ab = !wait_f(&cs.acc_full[b], (it >> 1) & 1, &cs.abort);
+                    ab = __any_sync(0xffffffffu, ab);
+                    if (ab) break;
+                    tc_fence_after();
+                    const uint32_t at = tl + (it & 1) * 256;
+                    it++;
+                    float v[2][16];  // the next 16 columns load while these are added
+                    tmem_ld16(at, v[0]);
+#pragma unroll
+                    for (int c = 0; c < BLK; c += 16) {
+                        tmem_wait_ld();
+                        if (c + 16 < BLK) {
+                            tmem_ld16(at + c + 16, v[(c / 16 + 1) & 1]);
+                        } else {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) arrive_cta0(&cs.acc_empty[b]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) fma2(acc[c + e], acc[c + e + 1], v[(c / 16) & 1] + e, s[i]);
+                    }
+                }
+            }
+            if (ab) {
+#pragma unroll
+                for (int c = 0; c < BLK; c++) acc[c] = __int_as_float(0x7fc00000);
+            }
+            if (EPI != STORE) {
+#pragma unroll
+                for (int c = 0; c < BLK; c++) acc[c] = acc[c] > 0.f ? acc[c] * acc[c] : (acc[c] == acc[c] ? 0.f : acc[c]);
+            }
+            float mul = 1.f;
+            if (EPI == RELU2_Q) {
+                float a = 0.f;
+#pragma unroll
+                for (int c = 0; c < BLK; c++) a = fmaxf(a, acc[c]);  // columns past N are 0
+                a = clamp_amax(a);
+                mul = quant_mul(a);
+                if (row0 + lane < un.rend && n0 < p.N) p.os[(long long)(n0 / BLK) * p.M + row0 + lane] = dequant_scale(a);
+            }
+            if (n0 >= p.N || row0 >= un.rend) continue;  // the same for the whole warp
+            constexpr int ES = sizeof(TO), PER = 16 / ES, BOX = 128 / ES;  // outputs in 16 and in 128 bytes
+            // the rows behind the last group's end are past the matrix, where the tensor map clips
+            const bool by_tma = tma_out && (row0 + 32 <= un.rend || un.rend == p.M);
+#pragma unroll
+            for (int c0 = 0; c0 < BLK; c0 += BOX) {
+                unsigned char* box = buf + (c0 / BOX % 2) * 4096;  // 32 rows x 128 bytes
+                if (c0 / BOX % 2 == 0) {  // the boxes' last stores have read them
+                    if (lane == 0) bulk_wait_read<0>();
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int q = 0; q < 8; q++)
+                    *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ lane) & 7) * 16) =
+                        pack_out<EPI, TO, PER>(&acc[c0 + q * PER], mul);
+                if (by_tma) {
+                    proxy_fence();
+                    __syncwarp();
+                    if (lane == 0 && n0 + c0 < p.N) tma_store_2d(&mo, n0 + c0, row0, box);
+                } else {
+                    __syncwarp();
+                    const int q = lane & 7, n = n0 + c0 + q * PER;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int r = i * 4 + (lane >> 3);
+                        const uint4 v = *reinterpret_cast<const uint4*>(box + r * 128 + ((q ^ r) & 7) * 16);
+                        const TO* e = reinterpret_cast<const TO*>(&v);
+                        TO* o = reinterpret_cast<TO*>(p.out) + (long long)(row0 + r) * p.ldo + n;
+                        if (row0 + r < un.rend) {
+                            if (tma_out && n + PER <= p.N) *reinterpret_cast<uint4*>(o) = v;
+                            else
+                                for (int j = 0; j < PER; j++)
+                                    if (n + j < p.N) o[j] = e[j];
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (lane == 0) bulk_wait_all();
+        __syncwarp();
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // no arrival and no MMA of the other CTA reaches this one any more
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+namespace fp8 {
+
+template <int EPI, typename TO>
+static int launch_pair(const GemmArgs& p, int pairs, cudaStream_t st) {
+    alignas(64) CUtensorMap ma, mw, mo;
+    if (map_a(&ma, p, BM) || map_w(&mw, p, 64)) return RWKV_ERR_CUDA;
+    constexpr int ES = sizeof(TO);
+    const int tma_out = aligned(p.out, 16) && (p.ldo * ES) % 16 == 0;  // else rows are stored one by one
+    if (tma_out) {
+        const cuuint64_t dims[2] = {(cuuint64_t)p.N, (cuuint64_t)p.M}, strides[1] = {(cuuint64_t)(p.ldo * ES)};
+        const cuuint32_t box[2] = {(cuuint32_t)(128 / ES), 32};
+        constexpr CUtensorMapDataType dt = ES == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                           : ES == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_UINT32;
+        if (make_map_dt(&mo, dt, p.out, 2, dims, strides, box, true)) return RWKV_ERR_CUDA;
+    } else {
+        mo = ma;
+    }
+    auto kern = fp8_gemm_pair_kernel<EPI, TO>;
+    const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM);
+    if (err != cudaSuccess) return set_cuda_error(err);
+    kern<<<2 * pairs, NTH, PAIR_SMEM, st>>>(ma, mw, mo, p, tma_out);
+    return check_launch();
+}
+
+static int gemm_pair(const GemmArgs& p, int epi, int out_dtype, int pairs, cudaStream_t st) {
+    if (epi == RELU2_Q) return launch_pair<RELU2_Q, uint8_t>(p, pairs, st);
+    RWKV_DISPATCH_DTYPE(out_dtype, TO, {
+        return epi == RELU2 ? launch_pair<RELU2, TO>(p, pairs, st) : launch_pair<STORE, TO>(p, pairs, st);
+    });
+    return RWKV_ERR_DTYPE;
+}
+
+}  // namespace fp8
+}  // namespace rwkv

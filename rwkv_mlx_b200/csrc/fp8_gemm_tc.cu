@@ -19,32 +19,19 @@
 // Every wait is bounded as in gemm_tc.cu: a wait that gives up sets the CTA's abort flag and
 // the device error word, the CTA's remaining outputs become NaN, copies and MMAs in flight
 // are drained before the tensor memory is freed.  No load uses cluster multicast.
-#include "fp8_gemm.cuh"
-#include "tma_common.cuh"
-#include "wkv7.cuh"
+#include "fp8_gemm_pair.cuh"
 
 namespace rwkv {
 
-__device__ int g_device_error_fp8;
-// Test hook (rwkv_debug_force_wait_timeout): every bounded wait gives up at once.
-static __constant__ int c_force_wait_timeout_fp8;
-
 namespace fp8 {
-using namespace tcc;
-using namespace tma;
 
-constexpr int BM = 128, NDRAIN = 256, NTH = NDRAIN + 128, MAXG = 256, CTRL = 4096;
-// A drain thread keeps BN / 2 sums and 32 loaded values, more than the 168 registers that 384
-// threads can have: the drain warpgroups take them from the third (setmaxnreg).
-constexpr int REG_LAUNCH = 168, REG_DRAIN = 216, REG_ISSUE = 72;
-static_assert(REG_DRAIN * NDRAIN + REG_ISSUE * (NTH - NDRAIN) <= REG_LAUNCH * NTH, "register split");
+constexpr int CTRL = 4096;
 
 struct Ctrl {
     unsigned long long full[8], empty[8], acc_full[2], acc_empty[2], drain;
     uint32_t tmem_base;
     int abort;
-    int goff[MAXG + 1];   // row offsets of the groups
-    int gunit[MAXG + 1];  // first unit of every group; [G] = number of units
+    Groups groups;
     float amax[2][BM];    // RELU2_Q with BN = 128: the two halves' maxima of each row
 };
 static_assert(sizeof(Ctrl) <= CTRL, "control block");
@@ -57,9 +44,6 @@ struct Cfg {
     static_assert(SMEM <= 227 * 1024 && NS <= 8, "shared memory");
 };
 
-__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int Nn) {  // fp32 accumulate, both e4m3, K-major
-    return (1u << 4) | ((uint32_t)(Nn >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
 __device__ __forceinline__ void umma8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
@@ -67,55 +51,6 @@ __device__ __forceinline__ void umma8(uint32_t d, uint64_t a, uint64_t b, uint32
         "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0), "r"(0), "r"(0), "r"(0)
         : "memory");
 }
-// Bounded wait; the first look is a bare try_wait, since the issuing thread's own instructions
-// are what bounds short blocks.
-__device__ __forceinline__ bool wait_f(unsigned long long* b, uint32_t parity, volatile int* abort) {
-    uint32_t ok;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                 : "=r"(ok)
-                 : "r"(ck::smem_u32(b)), "r"(parity)
-                 : "memory");
-    return ok || ck::mbar_wait(b, parity, abort, &g_device_error_fp8);
-}
-// a0 += s * v[0], a1 += s * v[1] in one packed instruction (same roundings as two fmaf).
-__device__ __forceinline__ void fma2(float& a0, float& a1, const float* v, float s) {
-    asm("{ .reg .b64 a, b, c; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %4}; mov.b64 c, {%0, %1}; "
-        "fma.rn.f32x2 c, a, b, c; mov.b64 {%0, %1}, c; }"
-        : "+f"(a0), "+f"(a1)
-        : "f"(v[0]), "f"(v[1]), "f"(s));
-}
-
-struct Unit {
-    int g, row0, rend, nt;
-};
-__device__ __forceinline__ Unit unit_of(const Ctrl& cs, int G, int ntn, int u) {
-    int lo = 0, hi = G;  // largest g with gunit[g] <= u (empty groups repeat a value)
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (cs.gunit[mid] <= u) lo = mid;
-        else hi = mid;
-    }
-    const int l = u - cs.gunit[lo];
-    return {lo, cs.goff[lo] + l / ntn * BM, cs.goff[lo + 1], l % ntn};
-}
-
-// 16 bytes of outputs from PER sums.
-template <int EPI, typename TO, int PER>
-__device__ __forceinline__ uint4 pack_out(const float* v, float mul) {
-    uint4 r;
-    if constexpr (EPI == RELU2_Q) {
-        r.x = pack4(v[0] * mul, v[1] * mul, v[2] * mul, v[3] * mul);
-        r.y = pack4(v[4] * mul, v[5] * mul, v[6] * mul, v[7] * mul);
-        r.z = pack4(v[8] * mul, v[9] * mul, v[10] * mul, v[11] * mul);
-        r.w = pack4(v[12] * mul, v[13] * mul, v[14] * mul, v[15] * mul);
-    } else {
-        TO* o = reinterpret_cast<TO*>(&r);
-#pragma unroll
-        for (int e = 0; e < PER; e++) o[e] = from_f32<TO>(v[e]);
-    }
-    return r;
-}
-
 // A warp's 32 rows x HC columns to memory.  A lane holds one row, so stores straight from
 // registers would write 16 bytes of 32 rows at a time (measured: 16,000 cycles for a 128 x 256
 // tile of 16-bit outputs, four times its products at K = 1024).  The warp turns 64-byte pieces
@@ -187,37 +122,14 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
         if (cs.abort) atomicOr(&g_device_error_fp8, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // offsets are clamped to [0, M]: rows outside the matrix belong to no tile
-    if (tid <= p.G) cs.goff[tid] = p.offs ? min(max(p.offs[tid], 0), p.M) : (tid == 0 ? 0 : p.M);
+    load_offsets(cs.groups, p, tid);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 0) {  // units per group (empty or negative groups: none), exclusive scan over the groups
-        constexpr int PER = (MAXG + 31) / 32;
-        int loc[PER], sum = 0;
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int g = lane * PER + i;
-            const int rows = g < p.G ? cs.goff[g + 1] - cs.goff[g] : 0;
-            loc[i] = sum;
-            sum += rows > 0 ? (rows + BM - 1) / BM * ntn : 0;
-        }
-        int incl = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += t;
-        }
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int g = lane * PER + i;
-            if (g < p.G) cs.gunit[g] = incl - sum + loc[i];
-        }
-        if (lane == 31) cs.gunit[p.G] = incl;
-    }
+    if (warp == 0) scan_units(cs.groups, p.G, BM, ntn, lane);
     __syncthreads();
     const uint32_t tmem = cs.tmem_base;
-    const int nunits = cs.gunit[p.G];
+    const int nunits = cs.groups.unit[p.G];
 
     if (warp >= NDRAIN / 32) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_ISSUE));
@@ -227,7 +139,7 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
                 int it = 0;
                 bool bad = false;
                 for (int u = blockIdx.x; u < nunits && !bad && !*(volatile int*)&cs.abort; u += gridDim.x) {
-                    const Unit un = unit_of(cs, p.G, ntn, u);
+                    const Unit un = unit_of(cs.groups, p.G, BM, ntn, u);
                     for (int kb = 0; kb < nk; kb++, it++) {
                         const int s = it % NS;
                         if (it >= NS && !wait_f(&cs.empty[s], ((it / NS) + 1) & 1, &cs.abort)) {
@@ -308,11 +220,11 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
             }
         };
         if ((int)blockIdx.x < nunits) {
-            aim(unit_of(cs, p.G, ntn, blockIdx.x));
+            aim(unit_of(cs.groups, p.G, BM, ntn, blockIdx.x));
             fetch(0);
         }
         for (int u = blockIdx.x; u < nunits; u += gridDim.x) {
-            const Unit un = unit_of(cs, p.G, ntn, u);
+            const Unit un = unit_of(cs.groups, p.G, BM, ntn, u);
             const int row = un.row0 + rl, n0 = un.nt * BN + half * HC, nb = n0 / BLK;
             const bool valid = row < un.rend;
             float acc[HC];
@@ -325,7 +237,7 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
                 if (kb0 + PF < nk) {
                     fetch(kb0 + PF);
                 } else if (u + (int)gridDim.x < nunits) {
-                    aim(unit_of(cs, p.G, ntn, u + gridDim.x));
+                    aim(unit_of(cs.groups, p.G, BM, ntn, u + gridDim.x));
                     fetch(0);
                 }
 #pragma unroll
@@ -394,27 +306,11 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
 
 namespace fp8 {
 
-static int sm_count() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n;
-}
-
 template <int BN, int EPI, typename TO>
 static int launch_tc(const GemmArgs& p, int grid, cudaStream_t st) {
     using C = Cfg<BN>;
     alignas(64) CUtensorMap ma, mw;
-    {
-        const cuuint64_t dims[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M}, strides[1] = {(cuuint64_t)p.lda};
-        const cuuint32_t box[2] = {(cuuint32_t)BLK, (cuuint32_t)BM};
-        if (make_map_dt(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.a, 2, dims, strides, box, true)) return RWKV_ERR_CUDA;
-    }
-    {
-        const cuuint64_t dims[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.G};
-        const cuuint64_t strides[2] = {(cuuint64_t)p.ldw, (cuuint64_t)(p.G > 1 ? p.gsw : (long long)p.N * p.ldw)};
-        const cuuint32_t box[3] = {(cuuint32_t)BLK, (cuuint32_t)BN, 1};
-        if (make_map_dt(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, 3, dims, strides, box, true)) return RWKV_ERR_CUDA;
-    }
+    if (map_a(&ma, p, BM) || map_w(&mw, p, BN)) return RWKV_ERR_CUDA;
     auto kern = fp8_gemm_tc_kernel<BN, EPI, TO>;
     const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (err != cudaSuccess) return set_cuda_error(err);
@@ -432,15 +328,12 @@ static int by_epi(const GemmArgs& p, int epi, int out_dtype, int grid, cudaStrea
     return RWKV_ERR_DTYPE;
 }
 
-// An upper bound of the row tiles of all groups that needs no offsets.
-static long long row_tiles(int M, int G) {
-    const long long most = (M + BM - 1) / BM + (G > 1 ? G - 1 : 0);
-    return most < M ? most : M;
-}
-
+int g_tc_impl = 0;
 int gemm_tc(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st) {
     const int sms = sm_count();
-    const long long mt = row_tiles(p.M, p.G), t256 = mt * ((p.N + 255) / 256), t128 = mt * ((p.N + 127) / 128);
+    const long long mt = row_tiles(p.M, p.G, BM), t256 = mt * ((p.N + 255) / 256), t128 = mt * ((p.N + 127) / 128);
+    const long long pairs = row_tiles(p.M, p.G, PM) * ((p.N + PN - 1) / PN);
+    if (g_tc_impl == 3) return gemm_pair(p, epi, out_dtype, (int)(pairs < sms / 2 ? pairs : sms / 2), st);
     if (t256 >= sms) return by_epi<256>(p, epi, out_dtype, (int)(t256 < sms ? t256 : sms), st);
     return by_epi<128>(p, epi, out_dtype, (int)(t128 < sms ? t128 : sms), st);
 }
