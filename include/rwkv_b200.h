@@ -374,8 +374,9 @@ int rwkv_fp8_experts(const void* x, long long ldx, const void* key, long long ld
                      const float* key_scale, const void* val, long long ldv, long long val_group_stride,
                      const float* val_scale, const int32_t* offs, void* out, long long ldo, void* workspace,
                      size_t workspace_bytes, int M, int C, int D, int E, int dtype, void* stream);
-/* Select the kernel of rwkv_fp8_gemm: 0 automatic, 1 mma.sync (streams the weights, for few
- * rows), 2 tcgen05.  Process-wide; meant for testing one against the other. */
+/* Select the kernel of the e4m3 products: 0 automatic, 1 mma.sync (streams the weights, for few
+ * rows), 2 tcgen05 with one CTA a tile, 3 tcgen05 by CTA pairs.  Process-wide; meant for testing
+ * one against the other. */
 int rwkv_fp8_set_gemm_impl(int impl);
 
 /* sum_{i<j} ||A_i^T A_j||_F^2 over the expert down-projections

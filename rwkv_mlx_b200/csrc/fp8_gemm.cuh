@@ -22,7 +22,7 @@ struct GemmArgs {
 };
 
 int gemm_stream(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st);
-int gemm_tc(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st);
+int gemm_tc(const GemmArgs& p, int epi, int out_dtype, int impl, cudaStream_t st);
 
 }  // namespace fp8
 }  // namespace rwkv

@@ -1,19 +1,20 @@
 // e4m3 products by CTA pairs (included by fp8_gemm_tc.cu): the method of that file on tiles of
 // 256 x 256, which one pair of SMs computes with cta_group::2 MMAs.  Each CTA loads 128 rows of A
 // and 128 rows of W a stage (32 KB instead of the 48 KB that a 128 x 256 tile needs for half the
-// products) and keeps 128 rows of the result.
+// products) and keeps 128 rows of the result.  Two accumulators of 256 columns fill tensor memory.
 //
-// A K block's product is issued as two MMA groups of 256 x 128, so that tensor memory holds four
-// accumulators of 128 columns: columns h * 128 .. + 127 of the tile belong to the drain warps of
-// half h, and an accumulator is refilled two blocks after it was handed over.
-//   warp 8 lane 0   producer: A (128 rows) and twice W (64 rows of each column half) by TMA,
-//                   signalled on the CTA's own "full" barrier;
-//   warp 9 lane 0   CTA 0: MMA issuer for the pair; CTA 1: forwards its "full" barriers to CTA 0
-//                   (a load here signals only its own CTA, so that each CTA can drain its own
-//                   copies when it has to give up);
-//   warps 0-7       drain and epilogue.  A warp lays its 32 x 128 outputs out in shared memory in
-//                   the tensor map's swizzle and hands them to TMA, which stores them while the
-//                   next tile is being computed; rows of another group's are guarded one by one.
+//   warp 8          producer: A (128 rows) and W (128 rows) by TMA;
+//   warp 9          CTA 0: MMA issuer for the pair, 4 MMAs (256 x 256 x 32) a block; CTA 1: forwards
+//                   its "full" barriers to CTA 0 (a load here signals only its own CTA, so that
+//                   CTA 1 can drain its own copies when it has to give up);
+//   warps 0-7       drain and epilogue, as in the one-CTA kernel.  A warp lays its 32 x 128 outputs out
+//                   in shared memory in the tensor map's swizzle and hands them to TMA, which stores
+//                   them while the next tile is being computed; where a tile ends inside another
+//                   group's rows, they are stored row by row.
+// As there, one wait and one commit a block for the issuing warp: CTA 0's "full" barrier of a
+// stage collects its own copies, CTA 1's forwarded arrival and the arrivals of the 16 drain warps
+// that have emptied the accumulator (with a barrier for each of these, and 256 x 128 MMAs on four
+// accumulators: 607 us at 16384 x 8192 x 4096 instead of 547).
 // Commits arrive in both CTAs (multicast of the arrival, not of data).
 #pragma once
 #include "fp8_tc.cuh"
@@ -22,11 +23,11 @@ namespace rwkv {
 namespace fp8 {
 
 constexpr int PM = 256, PN = 256, PNS = 5;
-constexpr int PA_BYTES = BM * BLK, PW_BYTES = 64 * BLK, PSTAGE = PA_BYTES + 2 * PW_BYTES;
+constexpr int PA_BYTES = BM * BLK, PSTAGE = 2 * PA_BYTES;
 constexpr int POUT = 8192;  // output staging of a drain warp
 
 struct PairCtrl {
-    unsigned long long full[PNS], empty[PNS], peer_full[PNS], acc_full[4], acc_empty[4], drain;
+    unsigned long long full[PNS], empty[PNS], acc_full[2], drain;
     uint32_t tmem_base;
     int abort;
     Groups groups;
@@ -49,37 +50,20 @@ __device__ __forceinline__ void commit_pair(unsigned long long* bar) {
         "h"((uint16_t)3)
         : "memory");
 }
-__device__ __forceinline__ void arrive_cta0(unsigned long long* bar) {
-    asm volatile(
-        "{ .reg .b32 ra; mapa.shared::cluster.u32 ra, %0, 0; "
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra]; }" ::"r"(ck::smem_u32(bar))
-        : "memory");
+// Arrive on the barrier at the same place in CTA 0.  What the arrival orders is tensor memory and
+// the async copies' data, not this thread's memory accesses, so the default (CTA) scope does; with
+// cluster scope it waited for the thread's outstanding loads (540 cycles a block).
+__device__ __forceinline__ uint32_t in_cta0(const unsigned long long* bar) {
+    uint32_t ra;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(ra) : "r"(ck::smem_u32(bar)));
+    return ra;
+}
+__device__ __forceinline__ void arrive_cta0(uint32_t ra) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(ra) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// wait_f for a barrier on which the other CTA arrives.
-__device__ __forceinline__ bool wait_c(unsigned long long* b, uint32_t parity, volatile int* abort) {
-    const uint32_t a = ck::smem_u32(b);
-    long long t0 = 0;
-    while (true) {
-        uint32_t ok;
-        asm volatile(
-            "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-            : "=r"(ok)
-            : "r"(a), "r"(parity)
-            : "memory");
-        if (ok) return true;
-        if (*abort) return false;
-        if (t0 == 0) t0 = clock64();
-        if (clock64() - t0 > ck::WAIT_CYCLES) {
-            *abort = 1;
-            atomicOr(&g_device_error_fp8, 1);
-            return false;
-        }
-    }
-}
-
 }  // namespace fp8
 
 template <int EPI, typename TO>
@@ -87,10 +71,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp8::NTH, 1)
     fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mw,
                          const __grid_constant__ CUtensorMap mo, const fp8::GemmArgs p, const int tma_out) {
     using namespace fp8;
-    constexpr uint32_t IDESC = idesc_e4m3(PM, 128);
+    constexpr uint32_t IDESC = idesc_e4m3(PM, PN);
 
     extern __shared__ __align__(1024) unsigned char smem_pair[];
-    unsigned char* ring = smem_pair;                       // stage: A box, W box of half 0, W box of half 1
+    unsigned char* ring = smem_pair;                       // stage: A box, W box (16 KB each)
     unsigned char* stage_out = ring + PNS * PSTAGE;        // 8 KB per drain warp
     PairCtrl& cs = *reinterpret_cast<PairCtrl*>(stage_out + NDRAIN / 32 * POUT);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -104,9 +88,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp8::NTH, 1)
     }
     if (tid == NDRAIN) {
         for (int i = 0; i < PNS; i++) {
-            ck::mbar_init(&cs.full[i], 1), ck::mbar_init(&cs.empty[i], 1), ck::mbar_init(&cs.peer_full[i], 1);
+            ck::mbar_init(&cs.full[i], rank == 0 ? 2 + 16 : 1);
+            ck::mbar_init(&cs.empty[i], 1);
         }
-        for (int i = 0; i < 4; i++) ck::mbar_init(&cs.acc_full[i], 1), ck::mbar_init(&cs.acc_empty[i], 8);
+        for (int i = 0; i < 2; i++) {
+            ck::mbar_init(&cs.acc_full[i], 1);
+            if (rank == 0)  // both accumulators start empty: the drain warps' arrivals for the first two blocks
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 16;" ::"r"(ck::smem_u32(&cs.full[i])) : "memory");
+        }
         ck::mbar_init(&cs.drain, 1);
         // the swizzle needs the ring on a 1024-byte boundary; nothing runs if it is not there
         cs.abort = c_force_wait_timeout_fp8 || (ck::smem_u32(ring) & 1023) ? 1 : 0;
@@ -125,82 +114,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp8::NTH, 1)
 
     if (warp >= NDRAIN / 32) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_ISSUE));
+        const bool el = elect_one();
+        int it = 0, s = 0;
+        uint32_t ph = 0;
+        bool bad = __any_sync(0xffffffffu, *(volatile int*)&cs.abort != 0);
         if (warp == NDRAIN / 32) {
             // ===================== producer =====================
-            if (lane == 0) {
-                int it = 0, s = 0;
-                uint32_t ph = 0;
-                bool bad = false;
-                for (int u = pair0; u < nunits && !bad && !*(volatile int*)&cs.abort; u += npairs) {
-                    const Unit un = unit_of(cs.groups, p.G, PM, ntn, u);
-                    const int row = un.row0 + rank * BM, n0 = un.nt * PN + rank * 64;
-                    for (int kb = 0; kb < nk; kb++, it++) {
-                        if (it >= PNS && !wait_f(&cs.empty[s], ph ^ 1, &cs.abort)) {
-                            bad = true;
-                            break;
-                        }
+            for (int u = pair0; u < nunits && !bad; u += npairs) {
+                const Unit un = unit_of(cs.groups, p.G, PM, ntn, u);
+                const int row = un.row0 + rank * BM, n0 = un.nt * PN + rank * 128;
+                for (int kb = 0; kb < nk; kb++, it++) {
+                    if (it >= PNS && !wait_w(&cs.empty[s], ph ^ 1, &cs.abort)) {
+                        bad = true;
+                        break;
+                    }
+                    if (el) {
                         unsigned char* st = ring + s * PSTAGE;
                         expect_tx(&cs.full[s], PSTAGE);
                         tma_load_2d(st, &ma, kb * BLK, row, &cs.full[s]);
                         tma_load_3d(st + PA_BYTES, &mw, kb * BLK, n0, un.g, &cs.full[s]);
-                        tma_load_3d(st + PA_BYTES + PW_BYTES, &mw, kb * BLK, n0 + 128, un.g, &cs.full[s]);
-                        if (++s == PNS) s = 0, ph ^= 1;
                     }
+                    if (++s == PNS) s = 0, ph ^= 1;
                 }
-                // shared memory stays allocated until the last copies have landed
-                for (int i = (it > PNS ? it - PNS : 0); i < it; i++)
-                    ck::mbar_drain(&cs.full[i % PNS], (i / PNS) & 1, &g_device_error_fp8);
             }
-            __syncwarp();
-        } else if (warp == NDRAIN / 32 + 1 && lane == 0) {
-            int it = 0, s = 0;
-            uint32_t ph = 0;
-            bool bad = false;
-            if (rank == 1) {
-                // ===================== forwarder =====================
-                for (int u = pair0; u < nunits && !bad && !*(volatile int*)&cs.abort; u += npairs)
-                    for (int kb = 0; kb < nk; kb++) {
-                        if (!wait_f(&cs.full[s], ph, &cs.abort)) {
-                            bad = true;
-                            break;
-                        }
-                        arrive_cta0(&cs.peer_full[s]);
-                        if (++s == PNS) s = 0, ph ^= 1;
+            // shared memory stays allocated until the last copies have landed (CTA 0 after a give-up:
+            // until the bound of this wait, since its barrier also collects others' arrivals)
+            for (int i = (it > PNS ? it - PNS : 0); i < it; i++)
+                ck::mbar_drain(&cs.full[i % PNS], (i / PNS) & 1, &g_device_error_fp8);
+        } else if (warp == NDRAIN / 32 + 1 && rank == 1) {
+            // ===================== forwarder =====================
+            const uint32_t peer = in_cta0(cs.full);
+            for (int u = pair0; u < nunits && !bad; u += npairs)
+                for (int kb = 0; kb < nk; kb++) {
+                    if (!wait_w(&cs.full[s], ph, &cs.abort)) {
+                        bad = true;
+                        break;
                     }
-            } else {
-                // ===================== MMA issuer =====================
-                const uint64_t desc_a = desc_sw128(ck::smem_u32(ring), 16, 1024);
-                for (int u = pair0; u < nunits && !bad && !*(volatile int*)&cs.abort; u += npairs)
-                    for (int kb = 0; kb < nk && !bad; kb++, it++) {
-                        if (!wait_f(&cs.full[s], ph, &cs.abort) || !wait_c(&cs.peer_full[s], ph, &cs.abort)) {
-                            bad = true;
-                            break;
-                        }
-                        const uint64_t da = desc_a + s * (PSTAGE >> 4);
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int b = (it & 1) * 2 + h;  // accumulator; refilled every second block
-                            if (it >= 2 && !wait_c(&cs.acc_empty[b], ((it >> 1) + 1) & 1, &cs.abort)) {
-                                bad = true;
-                                break;
-                            }
-                            tc_fence_after();
-#pragma unroll
-                            for (int kk = 0; kk < BLK / 32; kk++)
-                                umma8_pair(tmem + b * 128, da + kk * 2, da + ((PA_BYTES + h * PW_BYTES) >> 4) + kk * 2,
-                                           IDESC, kk > 0 ? 1u : 0u);
-                            commit_pair(&cs.acc_full[b]);
-                        }
-                        if (bad) break;
-                        commit_pair(&cs.empty[s]);
-                        if (++s == PNS) s = 0, ph ^= 1;
+                    if (el) arrive_cta0(peer + s * 8);
+                    if (++s == PNS) s = 0, ph ^= 1;
+                }
+        } else if (warp == NDRAIN / 32 + 1) {
+            // ===================== MMA issuer =====================
+            const uint64_t desc_a = desc_sw128(ck::smem_u32(ring), 16, 1024);
+            for (int u = pair0; u < nunits && !bad; u += npairs)
+                for (int kb = 0; kb < nk; kb++, it++) {
+                    if (!wait_w(&cs.full[s], ph, &cs.abort)) {
+                        bad = true;
+                        break;
                     }
-                // wait for this thread's own MMAs before either CTA's memory is freed
+                    tc_fence_after();
+                    const uint64_t da = desc_a + s * (PSTAGE >> 4);
+                    if (el) {
+#pragma unroll
+                        for (int kk = 0; kk < BLK / 32; kk++)
+                            umma8_pair(tmem + (it & 1) * PN, da + kk * 2, da + (PA_BYTES >> 4) + kk * 2, IDESC,
+                                       kk > 0 ? 1u : 0u);
+                        commit_pair(&cs.acc_full[it & 1]);
+                    }
+                    __syncwarp();
+                    if (++s == PNS) s = 0, ph ^= 1;
+                }
+            // wait for this thread's own MMAs before either CTA's memory is freed
+            if (el)
                 asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                                  ck::smem_u32(&cs.drain))
                              : "memory");
-                ck::mbar_drain(&cs.drain, 0, &g_device_error_fp8);
-            }
+            __syncwarp();
+            ck::mbar_drain(&cs.drain, 0, &g_device_error_fp8);
         }
         __syncwarp();
     } else {
@@ -211,6 +191,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp8::NTH, 1)
         const uint32_t tl = tmem + ((uint32_t)(32 * ew) << 16) + half * 128;
         const int nbn = (p.N + BLK - 1) / BLK;
         unsigned char* buf = stage_out + warp * POUT;
+        const uint32_t full0 = in_cta0(cs.full);
+        int se = 0, sf = 2;  // stages of this block and of the one that takes its accumulator next
         bool ab = *(volatile int*)&cs.abort != 0;
         int it = 0;
         // scales are loaded PF blocks at a time, one group of blocks ahead (fp8_gemm_tc_kernel)
@@ -253,12 +235,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp8::NTH, 1)
 #pragma unroll
                 for (int i = 0; i < PF; i++) {
                     if (kb0 + i >= nk || ab) break;
-                    const int b = (it & 1) * 2 + half;
-                    ab = !wait_f(&cs.acc_full[b], (it >> 1) & 1, &cs.abort);
+                    ab = !wait_f(&cs.acc_full[it & 1], (it >> 1) & 1, &cs.abort);
                     ab = __any_sync(0xffffffffu, ab);
                     if (ab) break;
                     tc_fence_after();
-                    const uint32_t at = tl + (it & 1) * 256;
+                    if (tid == 0) ck::mbar_arrive(&cs.empty[se]);
+                    if (++se == PNS) se = 0;
+                    const uint32_t at = tl + (it & 1) * PN;
                     it++;
                     float v[2][16];  // the next 16 columns load while these are added
                     tmem_ld16(at, v[0]);
@@ -270,7 +253,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp8::NTH, 1)
                         } else {
                             tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) arrive_cta0(&cs.acc_empty[b]);
+                            if (lane == 0) arrive_cta0(full0 + sf * 8);
+                            if (++sf == PNS) sf = 0;
                         }
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) fma2(acc[c + e], acc[c + e + 1], v[(c / 16) & 1] + e, s[i]);
@@ -351,7 +335,7 @@ namespace fp8 {
 template <int EPI, typename TO>
 static int launch_pair(const GemmArgs& p, int pairs, cudaStream_t st) {
     alignas(64) CUtensorMap ma, mw, mo;
-    if (map_a(&ma, p, BM) || map_w(&mw, p, 64)) return RWKV_ERR_CUDA;
+    if (map_a(&ma, p, BM) || map_w(&mw, p, 128)) return RWKV_ERR_CUDA;
     constexpr int ES = sizeof(TO);
     const int tma_out = aligned(p.out, 16) && (p.ldo * ES) % 16 == 0;  // else rows are stored one by one
     if (tma_out) {

@@ -3,19 +3,24 @@
 //   out[m, n] = epi( sum_kb as[kb, m] ws[g, n / 128, kb] sum_{k in block kb} a[m, k] w[g, n, k] )
 //
 // The scales change with every 128 values of K, so tensor memory holds only one K block's
-// sum at a time: the MMA warp writes block kb's 128 x BN product into one of two
-// accumulators (no accumulation across blocks), and the drain warps add it, times the row's
-// and the weight block's scale, to fp32 sums in registers while the other accumulator is
-// being written.  128 bytes of K are exactly one 128-byte swizzle row, so a pipeline stage
-// is one scale block.
-//   warp 8 lane 0   producer: A (128 x 128) and W (BN x 128) boxes by TMA into a ring;
-//   warp 9 lane 0   MMA issuer (warps 10 and 11 only give up their registers): 4 MMAs (128 x BN x 32) per block, commits to the stage's
-//                   "empty" barrier and the accumulator's "full" barrier;
+// sum at a time: the MMA warp writes block kb's product into one of NACC accumulators (no
+// accumulation across blocks), and the drain warps add it, times the row's and the weight
+// block's scale, to fp32 sums in registers while the other accumulators are being written.
+// 128 bytes of K are exactly one 128-byte swizzle row, so a pipeline stage is one scale block.
+//
+// This file: tiles of 128 x 128 by one CTA, for products with at most about one tile per SM, and
+// the choice between the kernels; fp8_gemm_pair.cuh: tiles of 256 x 256 by a CTA pair.
+//   warp 8          producer: A and W boxes (128 rows x 128 bytes each) by TMA into a ring;
+//   warp 9          MMA issuer: 4 MMAs (128 x 128 x 32) per block (warps 10 and 11 are idle);
 //   warps 0-7       drain: TMEM lane 32 (w % 4) + l = row of the tile, warps w and w + 4 take
 //                   the two column halves; one scale product per row and block.
-// The squared-ReLU expert's hidden rows are quantised in the epilogue: a thread holds one
-// row's columns, so a block's maximum is its own (BN = 256) or shared by two threads
-// (BN = 128).
+// The issuing warp's own time bounds a block (a wait takes it 190 cycles even when there is
+// nothing to wait for, a commit 70, four MMAs 50), so it waits and commits once a block: a
+// stage's "full" barrier collects the copies and the arrivals of the 8 drain warps that have
+// emptied the accumulator which the stage's products will go to, and the drain warps hand the
+// stage back to the producer once the accumulator's "full" barrier says its MMAs are done.
+// The squared-ReLU expert's hidden rows are quantised in the epilogue: two threads share a row's
+// 128 columns and exchange their maxima.
 // Every wait is bounded as in gemm_tc.cu: a wait that gives up sets the CTA's abort flag and
 // the device error word, the CTA's remaining outputs become NaN, copies and MMAs in flight
 // are drained before the tensor memory is freed.  No load uses cluster multicast.
@@ -25,24 +30,19 @@ namespace rwkv {
 
 namespace fp8 {
 
-constexpr int CTRL = 4096;
+constexpr int BN = 128, NACC = 4, NS = 6, CTRL = 4096;
+constexpr int A_BYTES = BM * BLK, STAGE = A_BYTES + BN * BLK;
+constexpr int SMEM = 1024 /* alignment slack */ + CTRL + NS * STAGE + NDRAIN / 32 * 2048;
+static_assert(SMEM <= 227 * 1024 && NACC < NS, "shared memory");
 
 struct Ctrl {
-    unsigned long long full[8], empty[8], acc_full[2], acc_empty[2], drain;
+    unsigned long long full[NS], empty[NS], acc_full[NACC], drain;
     uint32_t tmem_base;
     int abort;
     Groups groups;
-    float amax[2][BM];    // RELU2_Q with BN = 128: the two halves' maxima of each row
+    float amax[2][BM];  // RELU2_Q: the two halves' maxima of each row
 };
 static_assert(sizeof(Ctrl) <= CTRL, "control block");
-
-template <int BN>
-struct Cfg {
-    static constexpr int A_BYTES = BM * BLK, B_BYTES = BN * BLK, STAGE = A_BYTES + B_BYTES;
-    static constexpr int NS = BN == 256 ? 4 : 6;
-    static constexpr int SMEM = 1024 + CTRL + NS * STAGE + NDRAIN / 32 * 2048;
-    static_assert(SMEM <= 227 * 1024 && NS <= 8, "shared memory");
-};
 
 __device__ __forceinline__ void umma8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -91,32 +91,36 @@ __device__ __forceinline__ void store_rows(const GemmArgs& p, const float (&acc)
 
 }  // namespace fp8
 
-template <int BN, int EPI, typename TO>
+template <int EPI, typename TO>
 __global__ void __launch_bounds__(fp8::NTH, 1)
     fp8_gemm_tc_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mw,
                        const fp8::GemmArgs p, const int vec) {
     using namespace fp8;
-    using C = Cfg<BN>;
-    constexpr int NS = C::NS, HC = BN / 2;
-    constexpr uint32_t IDESC = idesc_e4m3(BM, BN), TCOLS = 2 * BN;
+    constexpr int HC = BN / 2;
+    constexpr uint32_t IDESC = idesc_e4m3(BM, BN);
 
     extern __shared__ __align__(1024) unsigned char smem_fp8_raw[];
     const uint32_t raw_addr = ck::smem_u32(smem_fp8_raw);
     unsigned char* smem = smem_fp8_raw + (((raw_addr + 1023) & ~1023u) - raw_addr);
     Ctrl& cs = *reinterpret_cast<Ctrl*>(smem);
-    unsigned char* ring = smem + CTRL;  // stage s: A box (16 KB) then W box (BN * 128 B), 1024-aligned
+    unsigned char* ring = smem + CTRL;  // stage s: A box then W box (16 KB each), 1024-aligned
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nk = (p.K + BLK - 1) / BLK, ntn = (p.N + BN - 1) / BN;
 
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ck::smem_u32(&cs.tmem_base)),
-                     "n"(TCOLS)
+                     "n"(NACC * BN)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (tid == NDRAIN) {
-        for (int i = 0; i < NS; i++) ck::mbar_init(&cs.full[i], 1), ck::mbar_init(&cs.empty[i], 1);
-        for (int i = 0; i < 2; i++) ck::mbar_init(&cs.acc_full[i], 1), ck::mbar_init(&cs.acc_empty[i], NDRAIN / 32);
+        for (int i = 0; i < NS; i++) ck::mbar_init(&cs.full[i], 1 + NDRAIN / 32), ck::mbar_init(&cs.empty[i], 1);
+        for (int i = 0; i < NACC; i++) {
+            ck::mbar_init(&cs.acc_full[i], 1);
+            // the accumulators start empty: the drain warps' arrivals for the first NACC blocks
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(ck::smem_u32(&cs.full[i])), "n"(NDRAIN / 32)
+                         : "memory");
+        }
         ck::mbar_init(&cs.drain, 1);
         cs.abort = c_force_wait_timeout_fp8 ? 1 : 0;
         if (cs.abort) atomicOr(&g_device_error_fp8, 2);
@@ -132,74 +136,66 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
     const int nunits = cs.groups.unit[p.G];
 
     if (warp >= NDRAIN / 32) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_ISSUE));
+        const bool el = elect_one();
+        int it = 0, s = 0;
+        uint32_t ph = 0;
+        bool bad = __any_sync(0xffffffffu, *(volatile int*)&cs.abort != 0);
         if (warp == NDRAIN / 32) {
             // ===================== producer =====================
-            if (lane == 0) {
-                int it = 0;
-                bool bad = false;
-                for (int u = blockIdx.x; u < nunits && !bad && !*(volatile int*)&cs.abort; u += gridDim.x) {
-                    const Unit un = unit_of(cs.groups, p.G, BM, ntn, u);
-                    for (int kb = 0; kb < nk; kb++, it++) {
-                        const int s = it % NS;
-                        if (it >= NS && !wait_f(&cs.empty[s], ((it / NS) + 1) & 1, &cs.abort)) {
-                            bad = true;
-                            break;
-                        }
-                        unsigned char* st = ring + s * C::STAGE;
-                        expect_tx(&cs.full[s], C::STAGE);
-                        tma_load_2d(st, &ma, kb * BLK, un.row0, &cs.full[s]);
-                        tma_load_3d(st + C::A_BYTES, &mw, kb * BLK, un.nt * BN, un.g, &cs.full[s]);
+            for (int u = blockIdx.x; u < nunits && !bad; u += gridDim.x) {
+                const Unit un = unit_of(cs.groups, p.G, BM, ntn, u);
+                for (int kb = 0; kb < nk; kb++, it++) {
+                    if (it >= NS && !wait_w(&cs.empty[s], ph ^ 1, &cs.abort)) {
+                        bad = true;
+                        break;
                     }
+                    if (el) {
+                        unsigned char* st = ring + s * STAGE;
+                        expect_tx(&cs.full[s], STAGE);
+                        tma_load_2d(st, &ma, kb * BLK, un.row0, &cs.full[s]);
+                        tma_load_3d(st + A_BYTES, &mw, kb * BLK, un.nt * BN, un.g, &cs.full[s]);
+                    }
+                    if (++s == NS) s = 0, ph ^= 1;
                 }
-                // the last NS copies may still be in flight: the shared memory they write must
-                // stay allocated until they have landed
-                for (int i = (it > NS ? it - NS : 0); i < it; i++)
-                    ck::mbar_drain(&cs.full[i % NS], (i / NS) & 1, &g_device_error_fp8);
             }
-            __syncwarp();
+            // shared memory stays allocated until the last copies have landed (after a give-up: until
+            // the bound of this wait, since the barriers also collect the drain warps' arrivals)
+            for (int i = (it > NS ? it - NS : 0); i < it; i++)
+                ck::mbar_drain(&cs.full[i % NS], (i / NS) & 1, &g_device_error_fp8);
         } else if (warp == NDRAIN / 32 + 1) {
             // ===================== MMA issuer =====================
-            if (lane == 0) {
-                // a descriptor's address field is bytes / 16 below 2^14: stages and K steps are added to it
-                const uint64_t desc_a = desc_sw128(ck::smem_u32(ring), 16, 1024);
-                int it = 0, s = 0;
-                uint32_t ph = 0;
-                bool bad = false;
-                for (int u = blockIdx.x; u < nunits && !bad && !*(volatile int*)&cs.abort; u += gridDim.x) {
-                    for (int kb = 0; kb < nk; kb++, it++) {
-                        const int acc = it & 1;
-                        if (!wait_f(&cs.full[s], ph, &cs.abort) ||
-                            (it >= 2 && !wait_f(&cs.acc_empty[acc], ((it >> 1) + 1) & 1, &cs.abort))) {
-                            bad = true;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint64_t da = desc_a + s * (C::STAGE >> 4);
+            // a descriptor's address field is bytes / 16 below 2^14: stages and K steps are added to it
+            const uint64_t desc_a = desc_sw128(ck::smem_u32(ring), 16, 1024);
+            for (int u = blockIdx.x; u < nunits && !bad; u += gridDim.x)
+                for (int kb = 0; kb < nk; kb++, it++) {
+                    if (!wait_w(&cs.full[s], ph, &cs.abort)) {
+                        bad = true;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t da = desc_a + s * (STAGE >> 4);
+                    if (el) {
 #pragma unroll
                         for (int kk = 0; kk < BLK / 32; kk++)
-                            umma8(tmem + acc * BN, da + kk * 2, da + (C::A_BYTES >> 4) + kk * 2, IDESC, kk > 0 ? 1u : 0u);
-                        umma_commit(&cs.empty[s]);
-                        umma_commit(&cs.acc_full[acc]);
-                        if (++s == NS) s = 0, ph ^= 1;
+                            umma8(tmem + it % NACC * BN, da + kk * 2, da + (A_BYTES >> 4) + kk * 2, IDESC, kk > 0 ? 1u : 0u);
+                        umma_commit(&cs.acc_full[it % NACC]);
                     }
+                    __syncwarp();
+                    if (++s == NS) s = 0, ph ^= 1;
                 }
-                if (it > 0) {  // wait for this thread's own MMAs before the memory is freed
-                    umma_commit(&cs.drain);
-                    ck::mbar_drain(&cs.drain, 0, &g_device_error_fp8);
-                }
-            }
+            if (el) umma_commit(&cs.drain);  // wait for this thread's own MMAs before the memory is freed
             __syncwarp();
+            ck::mbar_drain(&cs.drain, 0, &g_device_error_fp8);
         }
+        __syncwarp();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_DRAIN));
         // ===================== drain and epilogue =====================
         const int ew = warp & 3, half = warp >> 2;
         const int rl = 32 * ew + lane;  // row of the tile = TMEM lane
         const uint32_t tl = tmem + ((uint32_t)(32 * ew) << 16) + half * HC;
         const int nbn = (p.N + BLK - 1) / BLK;
         bool ab = *(volatile int*)&cs.abort != 0;
-        int it = 0;
+        int it = 0, se = 0, sf = NACC;  // stages of this block and of the one that takes its accumulator next
         // Scales come from L2 with a latency of one to two blocks' products, so they are loaded
         // PF blocks at a time, one group of blocks ahead (and a unit's first group before the
         // previous unit's outputs are stored).
@@ -243,13 +239,14 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
 #pragma unroll
                 for (int i = 0; i < PF; i++) {
                     if (kb0 + i >= nk || ab) break;
-                    const int b = it & 1;
-                    ab = !wait_f(&cs.acc_full[b], (it >> 1) & 1, &cs.abort);
+                    ab = !wait_f(&cs.acc_full[it % NACC], it / NACC & 1, &cs.abort);
                     ab = __any_sync(0xffffffffu, ab);
                     if (ab) break;
-                    it++;
                     tc_fence_after();
-                    const uint32_t at = tl + b * BN;
+                    if (tid == 0) ck::mbar_arrive(&cs.empty[se]);
+                    if (++se == NS) se = 0;
+                    const uint32_t at = tl + it % NACC * BN;
+                    it++;
                     float v[2][16];  // the next 16 columns load while these are added
                     tmem_ld16(at, v[0]);
 #pragma unroll
@@ -260,7 +257,8 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
                         } else {
                             tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) ck::mbar_arrive(&cs.acc_empty[b]);  // one arrival a warp: they serialise
+                            if (lane == 0) ck::mbar_arrive(&cs.full[sf]);  // one arrival a warp: they serialise
+                            if (++sf == NS) sf = 0;
                         }
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) fma2(acc[c + e], acc[c + e + 1], v[(c / 16) & 1] + e, s[i]);
@@ -280,18 +278,16 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
                 float a = 0.f;
 #pragma unroll
                 for (int c = 0; c < HC; c++) a = fmaxf(a, acc[c]);  // columns past N are 0
-                if (HC < BLK) {
-                    cs.amax[half][rl] = a;
-                    ck::bar_sync_n(1, NDRAIN);
-                    a = fmaxf(cs.amax[0][rl], cs.amax[1][rl]);
-                    ck::bar_sync_n(1, NDRAIN);
-                }
+                cs.amax[half][rl] = a;
+                ck::bar_sync_n(1, NDRAIN);
+                a = fmaxf(cs.amax[0][rl], cs.amax[1][rl]);
+                ck::bar_sync_n(1, NDRAIN);
                 a = clamp_amax(a);
                 mul = quant_mul(a);
                 if (valid && n0 < p.N && n0 % BLK == 0) p.os[(long long)nb * p.M + row] = dequant_scale(a);
             }
             if (n0 < p.N)
-                store_rows<EPI, HC, TO>(p, acc, ring + NS * C::STAGE + warp * 2048, un.row0 + 32 * ew,
+                store_rows<EPI, HC, TO>(p, acc, ring + NS * STAGE + warp * 2048, un.row0 + 32 * ew,
                                         un.rend - un.row0 - 32 * ew, n0, vec != 0, mul);
         }
     }
@@ -300,42 +296,41 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
     __syncthreads();
     if (warp == 0) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(TCOLS) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(NACC * BN) : "memory");
     }
 }
 
 namespace fp8 {
 
-template <int BN, int EPI, typename TO>
+template <int EPI, typename TO>
 static int launch_tc(const GemmArgs& p, int grid, cudaStream_t st) {
-    using C = Cfg<BN>;
     alignas(64) CUtensorMap ma, mw;
     if (map_a(&ma, p, BM) || map_w(&mw, p, BN)) return RWKV_ERR_CUDA;
-    auto kern = fp8_gemm_tc_kernel<BN, EPI, TO>;
-    const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    auto kern = fp8_gemm_tc_kernel<EPI, TO>;
+    const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (err != cudaSuccess) return set_cuda_error(err);
-    const int vec = aligned(p.out, 16) && (p.ldo * (EPI == RELU2_Q ? 1 : (int)sizeof(TO))) % 16 == 0;
-    kern<<<grid, NTH, C::SMEM, st>>>(ma, mw, p, vec);
+    const int vec = aligned(p.out, 16) && (p.ldo * (int)sizeof(TO)) % 16 == 0;
+    kern<<<grid, NTH, SMEM, st>>>(ma, mw, p, vec);
     return check_launch();
 }
 
-template <int BN>
-static int by_epi(const GemmArgs& p, int epi, int out_dtype, int grid, cudaStream_t st) {
-    if (epi == RELU2_Q) return launch_tc<BN, RELU2_Q, uint8_t>(p, grid, st);
+// impl: 0 automatic, 2 one CTA a tile, 3 CTA pairs.  Measured, us, one CTA / pair: 1024 x 1024 x 1024
+// 6.9 / 9.7, 4096 x 1024 x 1024 (256 tiles) 11.4 / 10.2, 8192 x 4096 x 1024 55 / 43; 64 groups of
+// N = 2048, K = 1024 with 128 rows on average 51 / 64, with 512 rows 133 / 120.  So a pair once the
+// small tiles exceed the SMs, and where groups are at least a pair's tile and a half long.
+int gemm_tc(const GemmArgs& p, int epi, int out_dtype, int impl, cudaStream_t st) {
+    const int sms = sm_count();
+    const long long tiles = row_tiles(p.M, p.G, BM) * ((p.N + BN - 1) / BN);
+    const long long pairs = row_tiles(p.M, p.G, PM) * ((p.N + PN - 1) / PN);
+    const bool pair = tiles > sms && (p.G == 1 || p.M / p.G >= PM * 3 / 2);
+    if (impl == 3 || (impl == 0 && pair))
+        return gemm_pair(p, epi, out_dtype, (int)(pairs < sms / 2 ? pairs : sms / 2), st);
+    const int grid = (int)(tiles < sms ? tiles : sms);
+    if (epi == RELU2_Q) return launch_tc<RELU2_Q, uint8_t>(p, grid, st);
     RWKV_DISPATCH_DTYPE(out_dtype, TO, {
-        return epi == RELU2 ? launch_tc<BN, RELU2, TO>(p, grid, st) : launch_tc<BN, STORE, TO>(p, grid, st);
+        return epi == RELU2 ? launch_tc<RELU2, TO>(p, grid, st) : launch_tc<STORE, TO>(p, grid, st);
     });
     return RWKV_ERR_DTYPE;
-}
-
-int g_tc_impl = 0;
-int gemm_tc(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st) {
-    const int sms = sm_count();
-    const long long mt = row_tiles(p.M, p.G, BM), t256 = mt * ((p.N + 255) / 256), t128 = mt * ((p.N + 127) / 128);
-    const long long pairs = row_tiles(p.M, p.G, PM) * ((p.N + PN - 1) / PN);
-    if (g_tc_impl == 3) return gemm_pair(p, epi, out_dtype, (int)(pairs < sms / 2 ? pairs : sms / 2), st);
-    if (t256 >= sms) return by_epi<256>(p, epi, out_dtype, (int)(t256 < sms ? t256 : sms), st);
-    return by_epi<128>(p, epi, out_dtype, (int)(t128 < sms ? t128 : sms), st);
 }
 
 }  // namespace fp8

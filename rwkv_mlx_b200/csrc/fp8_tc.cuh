@@ -1,5 +1,6 @@
 // Shared by the tcgen05 e4m3 products (fp8_gemm_tc.cu: one CTA a tile, fp8_gemm_pair.cuh: a
-// CTA pair a tile; both are one translation unit with one device error word): sizes, the group table, packed adds and output packing.
+// CTA pair a tile; both are one translation unit with one device error word): sizes, the group
+// table, packed adds and output packing.
 #pragma once
 #include "fp8_gemm.cuh"
 #include "tma_common.cuh"
@@ -16,8 +17,8 @@ using namespace tcc;
 using namespace tma;
 
 constexpr int BM = 128, NDRAIN = 256, NTH = NDRAIN + 128, MAXG = 256;
-// A drain thread keeps BN / 2 sums and 32 loaded values, more than the 168 registers that 384
-// threads can have: the drain warpgroups take them from the third (setmaxnreg).
+// A pair kernel's drain thread keeps 128 sums and 32 loaded values, more than the 168 registers that
+// 384 threads can have: the drain warpgroups take them from the third (setmaxnreg).
 constexpr int REG_LAUNCH = 168, REG_DRAIN = 216, REG_ISSUE = 72;
 static_assert(REG_DRAIN * NDRAIN + REG_ISSUE * (NTH - NDRAIN) <= REG_LAUNCH * NTH, "register split");
 
@@ -34,6 +35,19 @@ __device__ __forceinline__ bool wait_f(unsigned long long* b, uint32_t parity, v
                  : "r"(ck::smem_u32(b)), "r"(parity)
                  : "memory");
     return ok || ck::mbar_wait(b, parity, abort, &g_device_error_fp8);
+}
+
+// One lane of a converged warp.  The issuing warps run their loops as a whole and only the
+// asynchronous instructions under this predicate: descriptors and addresses then stay in uniform
+// registers (issued from a one-lane branch, four MMAs took 260 cycles instead of 50).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(ok));
+    return ok != 0;
+}
+// wait_f by a whole warp, with the same answer for all lanes.
+__device__ __forceinline__ bool wait_w(unsigned long long* b, uint32_t parity, volatile int* abort) {
+    return __all_sync(0xffffffffu, wait_f(b, parity, abort));
 }
 
 // a0 += s * v[0], a1 += s * v[1] in one packed instruction (same roundings as two fmaf).
