@@ -3,7 +3,8 @@
 Drop-in replacements for the hot paths of RWKV-MLX (rwkv_mlx/kernels/wkv7_metal.py,
 rwkv_mlx/model.py, rwkv_mlx/moe.py) on hand-written CUDA kernels behind the C ABI
 declared in include/rwkv_b200.h.  Submodules: ``wkv7`` (WKV-7 operators),
-``moe`` (Router / LoRAMoE_CMix), ``model`` (the RWKV-v7 model shell), ``ep``
+``moe`` (Router / LoRAMoE_CMix / Fp8MoE_CMix), ``route`` (routing to experts from logits),
+``fp8`` (products in 8-bit floating point), ``model`` (the RWKV-v7 model shell), ``ep``
 (expert-parallel dispatch / combine).
 """
 

@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(NT, EPL <= 8 ? 4 : 2) route_kernel(const Args 
             } else if (on) {
                 s = z == 0.f ? 0.f : expf(lj - m) / z;
             }
+            if (on && !by_logit) s += z - z;  // a NaN logit anywhere makes every score of the row NaN
         }
         if (p.renorm) {
             const float sum = wsum(s);

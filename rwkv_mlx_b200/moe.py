@@ -22,9 +22,13 @@ products of each expert run as library GEMMs (cuBLAS) on that expert's contiguou
 range with the squared ReLU applied in place between them (``rwkv_relu_sq``), and
 ``rwkv_moe_combine_rows`` forms the score-weighted sum per token.
 
-These modules compute the forward pass only (no autograd through the kernels): a call
-with autograd enabled that would need gradients (an input that requires grad, or a
-trainable adapter / router / expert parameter) raises instead of returning values
+:class:`Fp8MoE_CMix` serves the same experts with their weights in e4m3, and
+:class:`GroupRouter` routes over many experts (sigmoid scores, balance bias, groups);
+both are additions without a counterpart in the reference.
+
+These modules, :class:`GroupRouter` apart, compute the forward pass only (no autograd
+through the kernels): a call with autograd enabled that would need gradients (an input
+that requires grad, or a trainable adapter / router / expert parameter) raises instead of returning values
 that silently carry no gradient.  Run them under ``torch.no_grad()`` /
 ``torch.inference_mode()``, or freeze the parameters.
 """
@@ -37,7 +41,9 @@ import torch
 from torch import nn
 
 from . import _native as nat
+from .fp8 import fp8_experts, quantize_fp8_weight
 from .fused import grouped_gemm, relu_sq_
+from .route import route_experts, update_balance_bias
 
 
 def _stream(dev):
@@ -261,6 +267,36 @@ class Router(nn.Module):
                 r["aux"], r["z"])
 
 
+class GroupRouter(nn.Module):
+    """Router for many experts: sigmoid or softmax scores, a bias that balances the load, selection
+    within the best groups of experts (:func:`rwkv_mlx_b200.route.route_experts`).  No counterpart in
+    the reference, whose :class:`Router` balances by the auxiliary losses instead.
+
+    The gate product runs in fp32.  Differentiable in ``x`` and ``gate.weight``; ``balance_bias`` is a
+    buffer that only :meth:`update_balance` moves."""
+
+    def __init__(self, d_model: int, n_experts: int, top_k: int = 2, *, score: str = "sigmoid", n_groups: int = 1,
+                 topk_groups: int = 1, group_score: str = "top2", renormalize: bool = True, scale: float = 1.0,
+                 balance: bool = True):
+        super().__init__()
+        self.gate = nn.Linear(d_model, n_experts, bias=False)
+        self.n_experts, self.top_k = n_experts, top_k
+        self.opts = dict(score=score, n_groups=n_groups, topk_groups=topk_groups, group_score=group_score,
+                         renormalize=renormalize, scale=scale)
+        self.register_buffer("balance_bias", torch.zeros(n_experts) if balance else None)
+
+    def forward(self, x: torch.Tensor):
+        """x (..., C) -> (inds (..., k) int32, weights (..., k) fp32, counts (E,) int32)."""
+        logits = nn.functional.linear(x.to(torch.float32), self.gate.weight.to(torch.float32))
+        return route_experts(logits, self.top_k, bias=self.balance_bias, return_counts=True, **self.opts)
+
+    def update_balance(self, counts: torch.Tensor, rate: float = 1e-3) -> None:
+        """After a training step: raise the bias of experts with less than the mean load, lower the others'."""
+        if self.balance_bias is None:
+            raise RuntimeError("GroupRouter: built without a balance bias")
+        update_balance_bias(self.balance_bias, counts, rate)
+
+
 class LoRAMoE_CMix(nn.Module):
     """ChannelMix with LoRA expert adapters on a shared frozen base (moe.py:93-163).
 
@@ -383,3 +419,57 @@ class MoE_CMix(nn.Module):
     def orthogonal_loss(self) -> torch.Tensor:
         """No orthogonality loss for full experts (moe.py:241-242)."""
         return torch.zeros((), device=self.x_k.device, dtype=torch.float32)
+
+
+class Fp8MoE_CMix(nn.Module):
+    """A :class:`MoE_CMix` (moe.py:170-242) served with its expert weights in e4m3, one fp32 scale for
+    each 128 x 128 block: half the bytes of the 16-bit experts and the tensor cores' 8-bit rate.
+
+    ``Fp8MoE_CMix(moe)`` quantises the experts once and keeps the module's own router;
+    ``Fp8MoE_CMix(moe, router)`` takes a :class:`GroupRouter`.  Calls and shapes are MoE_CMix's; forward
+    only.  The rows of each expert are quantised per 128 channels, its hidden rows in the key product's
+    kernel (:func:`rwkv_mlx_b200.fp8.fp8_experts`)."""
+
+    def __init__(self, moe: MoE_CMix, router: nn.Module | None = None):
+        super().__init__()
+        self.n_experts, self.top_k, self.layer_id = moe.n_experts, moe.top_k, moe.layer_id
+        self.router = moe.router if router is None else router
+        if self.router.n_experts != self.n_experts:
+            raise ValueError(f"Fp8MoE_CMix: the router has {self.router.n_experts} experts, the layer {self.n_experts}")
+        self.register_buffer("x_k", moe.x_k.detach().clone())
+        for name, w in (("key", moe.expert_key), ("val", moe.expert_val)):
+            q, s = quantize_fp8_weight(w)
+            # bytes and bits, so that Module.half() and the like do not convert them
+            self.register_buffer(f"expert_{name}", q.view(torch.uint8))
+            self.register_buffer(f"expert_{name}_scale", s.view(torch.int32))
+
+    def expert_weights(self):
+        """(key, key_scale, val, val_scale) as :func:`rwkv_mlx_b200.fp8.fp8_experts` takes them."""
+        return (self.expert_key.view(torch.float8_e4m3fn), self.expert_key_scale.view(torch.float32),
+                self.expert_val.view(torch.float8_e4m3fn), self.expert_val_scale.view(torch.float32))
+
+    def _experts(self, x2d: torch.Tensor, prev, T: int):
+        ntok, _ = x2d.shape
+        zero = torch.zeros((), device=x2d.device)
+        if isinstance(self.router, GroupRouter):
+            inds, weights, _ = self.router(x2d)
+            weights, aux, z = weights.to(x2d.dtype), zero, zero
+        else:
+            r = router_forward(x2d, self.router.gate.weight, self.router.top_k, self.router.bias)
+            inds, weights, aux, z = r["inds"], r["scores"], r["aux"], r["z"]
+        perm, inv, offsets = permute(inds, self.n_experts)
+        rows = expert_mix_rows(x2d, prev, self.x_k, perm, offsets, T, inds.shape[1])
+        out = fp8_experts(rows, *self.expert_weights(), offsets)
+        return combine_rows(None, out, weights, inv, ntok), aux, z
+
+    def forward(self, x: torch.Tensor):
+        """x (B, T, C) -> (out (B, T, C), aux_loss, z_loss); both losses 0 with a GroupRouter."""
+        check_forward_only("Fp8MoE_CMix", x, self.parameters())
+        B, T, C = x.shape
+        out, aux, z = self._experts(x.reshape(B * T, C).contiguous(), None, T)
+        return out.reshape(B, T, C), aux, z
+
+    def forward_rnn(self, x: torch.Tensor, x_prev: torch.Tensor) -> torch.Tensor:
+        """One token per sequence: x, x_prev (Bs, C) -> (Bs, C), as MoE_CMix.forward_rnn."""
+        check_forward_only("Fp8MoE_CMix", x, self.parameters())
+        return self._experts(x.contiguous(), x_prev, 1)[0]
