@@ -29,6 +29,15 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
     return pack2(a, b) | (pack2(c, d) << 16);
 }
 
+// relu(x)^2, a NaN kept.  One max that propagates NaN, no selection: written as a comparison the
+// compiler branched for each of a thread's 128 sums (380 us against 236 for a key product of
+// 32768 rows, N = 4096, K = 1024).
+__device__ __forceinline__ float relu_sq(float x) {
+    float y;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+    return y * y;
+}
+
 // 8 consecutive values as floats (16-byte aligned).
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&o)[8]) {

@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(SNT) gemm_stream_kernel(const GemmArgs p) {
                 float v = 0.f;
 #pragma unroll
                 for (int w = 0; w < SNW; w++) v += red[w][n][i / SROWS];
-                if (RELU2) v = v > 0.f ? v * v : (v == v ? 0.f : v);
+                if (RELU2) v = relu_sq(v);
                 reinterpret_cast<TO*>(p.out)[(long long)m * p.ldo + n0 + n] = from_f32<TO>(v);
             }
         }

@@ -267,7 +267,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp8::NTH, 1)
             }
             if (EPI != STORE) {
 #pragma unroll
-                for (int c = 0; c < BLK; c++) acc[c] = acc[c] > 0.f ? acc[c] * acc[c] : (acc[c] == acc[c] ? 0.f : acc[c]);
+                for (int c = 0; c < BLK; c++) acc[c] = relu_sq(acc[c]);
             }
             float mul = 1.f;
             if (EPI == RELU2_Q) {

@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
             }
             if (EPI != STORE) {
 #pragma unroll
-                for (int c = 0; c < HC; c++) acc[c] = acc[c] > 0.f ? acc[c] * acc[c] : (acc[c] == acc[c] ? 0.f : acc[c]);
+                for (int c = 0; c < HC; c++) acc[c] = relu_sq(acc[c]);
             }
             float mul = 1.f;
             if (EPI == RELU2_Q) {
