@@ -14,7 +14,7 @@
 namespace rwkv {
 namespace fp8 {
 
-constexpr int SNT = 256, SNW = SNT / 32, SROWS = 16;
+constexpr int SROWS = 16;
 
 __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -23,10 +23,16 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// 16 bytes of a row from k on; bytes past K are 0 (never read).
-__device__ __forceinline__ uint4 load16(const uint8_t* row, int k, int K, bool on) {
-    uint4 r = make_uint4(0u, 0u, 0u, 0u);
-    if (!on || k >= K) return r;
+// 16 bytes of a row from k on, 0 past K.  VEC: K is a multiple of 16, so a piece is all in the row
+// or all past it and the load needs no branch; else the last piece is read byte by byte.
+template <bool VEC>
+__device__ __forceinline__ uint4 load16(const uint8_t* row, int k, int K) {
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    if (VEC) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + (k < K ? k : 0)));
+        return k < K ? v : zero;
+    }
+    if (k >= K) return zero;
     if (k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
     uint32_t v[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
@@ -35,64 +41,131 @@ __device__ __forceinline__ uint4 load16(const uint8_t* row, int k, int K, bool o
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-template <typename TO, int NT8, bool RELU2>
-__global__ void __launch_bounds__(SNT) gemm_stream_kernel(const GemmArgs p) {
-    constexpr int TP = 8 * NT8;
-    __shared__ float red[SNW][SROWS][TP + 1];
+struct Quantised {};  // the rows are e4m3 already
+
+// NW warps, RT 16-row tiles of W a CTA, 8 NT8 tokens a pass.  TX: Quantised, or the type of rows that the
+// CTA quantises itself into shared memory (8 tokens a pass, the formulas of fp8_common.cuh): for a few
+// tokens that is less than a launch of its own, and the weights' first loads cover it (4 tokens,
+// 4096 x 1024: 3.5 us against 4.7 in two launches).
+template <typename TO, typename TX, int NW, int RT, int NT8, bool VEC, bool RELU2>
+__global__ void __launch_bounds__(NW * 32) gemm_stream_kernel(const GemmArgs p) {
+    constexpr bool SELF = !std::is_same<TX, Quantised>::value;
+    static_assert(!SELF || (NT8 == 1 && VEC), "tokens are quantised 8 at a time");
+    constexpr int TP = 8 * NT8, ROWS = SROWS * RT;
+    __shared__ float red[NW][ROWS][TP + 1];
+    extern __shared__ __align__(16) unsigned char smem_stream[];  // SELF: 8 token rows, then their scales
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
-    const int g = blockIdx.y, n0 = blockIdx.x * SROWS;
+    const int g = blockIdx.y, n0 = blockIdx.x * ROWS;
     const int r0 = p.offs ? max(p.offs[g], 0) : 0, r1 = p.offs ? min(p.offs[g + 1], p.M) : p.M;
+    if (r0 >= r1) return;
     const int nkb = (p.K + BLK - 1) / BLK;
+    const int pitch = nkb * BLK + 16;  // eight rows' pieces of one column lie in different banks
+    float* tscale = reinterpret_cast<float*>(smem_stream + 8 * pitch);
+    // a CTA's rows lie in one 128-row block of W: 128 is a multiple of ROWS
     const float* wsb = p.ws + ((long long)g * ((p.N + BLK - 1) / BLK) + n0 / BLK) * nkb;
-    const uint8_t* w0 = p.w + (long long)g * p.gsw + (long long)(n0 + gr) * p.ldw;
-    const uint8_t* w1 = w0 + 8 * p.ldw;
-    const bool on0 = n0 + gr < p.N, on1 = n0 + gr + 8 < p.N;
+    const uint8_t* w[RT][2];  // rows past N read the last one; their results are not stored
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            w[r][i] = p.w + (long long)g * p.gsw + (long long)min(n0 + 16 * r + 8 * i + gr, p.N - 1) * p.ldw;
     for (int m0 = r0; m0 < r1; m0 += TP) {
-        float acc[NT8][4];
+        const uint8_t* a[NT8];  // tokens past the group read its last one; their scale is 0
 #pragma unroll
         for (int j = 0; j < NT8; j++)
+            a[j] = SELF ? smem_stream + min(gr, r1 - m0 - 1) * pitch : p.a + (long long)min(m0 + 8 * j + gr, r1 - 1) * p.lda;
+        uint4 wv[RT][2][2], av[NT8][2];  // all of a block's loads are on their way before the first product
+        float s[NT8][2], sb = 0.f, acc[RT][NT8][4];
+        auto load_w = [&](int kb) {
+            sb = __ldg(wsb + kb);
 #pragma unroll
-            for (int c = 0; c < 4; c++) acc[j][c] = 0.f;
-        for (int kb = warp; kb < nkb; kb += SNW) {
-            const float sb = wsb[kb];
-            float part[NT8][4];
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int r = 0; r < RT; r++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) wv[r][i][h] = load16<VEC>(w[r][i], kb * BLK + h * 64 + t * 16, p.K);
+        };
+        auto load_a = [&](int kb) {
+#pragma unroll
+            for (int j = 0; j < NT8; j++) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int k = kb * BLK + h * 64 + t * 16;
+                    if constexpr (SELF) av[j][h] = *reinterpret_cast<const uint4*>(a[j] + k);
+                    else av[j][h] = load16<VEC>(a[j], k, p.K);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int m = m0 + 8 * j + 2 * t + i;
+                    s[j][i] = m >= r1 ? 0.f : SELF ? tscale[(2 * t + i) * nkb + kb] : __ldg(p.as + (long long)kb * p.M + m);
+                }
+            }
+        };
+#pragma unroll
+        for (int r = 0; r < RT; r++)
 #pragma unroll
             for (int j = 0; j < NT8; j++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) part[j][c] = 0.f;
+                for (int c = 0; c < 4; c++) acc[r][j][c] = 0.f;
+        if constexpr (SELF) {
+            if (warp < nkb) load_w(warp);
+            const int ntok = min(8, r1 - m0), l = lane & 15;
+            for (int b0 = 2 * warp; b0 < ntok * nkb; b0 += 2 * NW) {  // a block a half-warp
+                const int b = b0 + (lane >> 4), tok = b / nkb, kb = b % nkb, k = kb * BLK + l * 8;
+                const bool on = b < ntok * nkb;
+                float v[8], top = 0.f;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int k = kb * BLK + h * 64 + t * 16;
-                const uint4 a0 = load16(w0, k, p.K, on0), a1 = load16(w1, k, p.K, on1);
+                for (int e = 0; e < 8; e++) v[e] = 0.f;
+                if (on && k < p.K) load8(reinterpret_cast<const TX*>(p.x) + (long long)(m0 + tok) * p.ldx + k, v);
 #pragma unroll
-                for (int j = 0; j < NT8; j++) {
-                    const int m = m0 + 8 * j + gr;
-                    const uint4 b = load16(p.a + (long long)m * p.lda, k, p.K, m < r1);
-                    mma_e4m3(part[j], a0.x, a1.x, a0.y, a1.y, b.x, b.y);
-                    mma_e4m3(part[j], a0.z, a1.z, a0.w, a1.w, b.z, b.w);
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(v[e]));
+#pragma unroll
+                for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top = clamp_amax(top);
+                const float mul = quant_mul(top);
+                if (on) {
+                    uint2 q;
+                    q.x = pack4(v[0] * mul, v[1] * mul, v[2] * mul, v[3] * mul);
+                    q.y = pack4(v[4] * mul, v[5] * mul, v[6] * mul, v[7] * mul);
+                    *reinterpret_cast<uint2*>(smem_stream + tok * pitch + k) = q;
+                    if (l == 0) tscale[tok * nkb + kb] = dequant_scale(top);
                 }
             }
+            __syncthreads();
+        }
+        for (int kb = warp; kb < nkb; kb += NW) {
+            if (!SELF || kb != warp) load_w(kb);
+            load_a(kb);
 #pragma unroll
-            for (int j = 0; j < NT8; j++) {
-                const int m = m0 + 8 * j + 2 * t;
-                const float s0 = m < r1 ? p.as[(long long)kb * p.M + m] * sb : 0.f;
-                const float s1 = m + 1 < r1 ? p.as[(long long)kb * p.M + m + 1] * sb : 0.f;
-                acc[j][0] += part[j][0] * s0, acc[j][1] += part[j][1] * s1;
-                acc[j][2] += part[j][2] * s0, acc[j][3] += part[j][3] * s1;
-            }
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int j = 0; j < NT8; j++) {
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint4 x = wv[r][0][h], y = wv[r][1][h], b = av[j][h];
+                        mma_e4m3(part, x.x, y.x, x.y, y.y, b.x, b.y);
+                        mma_e4m3(part, x.z, y.z, x.w, y.w, b.z, b.w);
+                    }
+                    const float s0 = s[j][0] * sb, s1 = s[j][1] * sb;
+                    acc[r][j][0] += part[0] * s0, acc[r][j][1] += part[1] * s1;
+                    acc[r][j][2] += part[2] * s0, acc[r][j][3] += part[3] * s1;
+                }
         }
 #pragma unroll
-        for (int j = 0; j < NT8; j++) {
-            red[warp][gr][8 * j + 2 * t] = acc[j][0], red[warp][gr][8 * j + 2 * t + 1] = acc[j][1];
-            red[warp][gr + 8][8 * j + 2 * t] = acc[j][2], red[warp][gr + 8][8 * j + 2 * t + 1] = acc[j][3];
-        }
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int j = 0; j < NT8; j++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    red[warp][16 * r + gr + 8 * (c >> 1)][8 * j + 2 * t + (c & 1)] = acc[r][j][c];
         __syncthreads();
-        for (int i = threadIdx.x; i < SROWS * TP; i += SNT) {
-            const int m = m0 + i / SROWS, n = i % SROWS;
+        for (int i = threadIdx.x; i < ROWS * TP; i += NW * 32) {
+            const int m = m0 + i / ROWS, n = i % ROWS;
             if (m < r1 && n0 + n < p.N) {
                 float v = 0.f;
 #pragma unroll
-                for (int w = 0; w < SNW; w++) v += red[w][n][i / SROWS];
+                for (int q = 0; q < NW; q++) v += red[q][n][i / ROWS];
                 if (RELU2) v = relu_sq(v);
                 reinterpret_cast<TO*>(p.out)[(long long)m * p.ldo + n0 + n] = from_f32<TO>(v);
             }
@@ -101,19 +174,47 @@ __global__ void __launch_bounds__(SNT) gemm_stream_kernel(const GemmArgs p) {
     }
 }
 
-template <typename TO, bool RELU2>
-static int stream_launch(const GemmArgs& p, cudaStream_t st) {
-    const dim3 grid((p.N + SROWS - 1) / SROWS, p.G);
-    // 8 tokens a pass when a group has at most about that many rows, else 32
-    if ((long long)p.M <= 8LL * p.G) gemm_stream_kernel<TO, 1, RELU2><<<grid, SNT, 0, st>>>(p);
-    else gemm_stream_kernel<TO, 4, RELU2><<<grid, SNT, 0, st>>>(p);
+template <typename TO, typename TX, int NW, int RT, int NT8, bool RELU2>
+static int stream_launch_t(const GemmArgs& p, cudaStream_t st) {
+    const dim3 grid((p.N + SROWS * RT - 1) / (SROWS * RT), p.G);
+    if constexpr (!std::is_same<TX, Quantised>::value) {
+        const int nkb = (p.K + BLK - 1) / BLK, smem = 8 * (nkb * BLK + 16) + 8 * nkb * (int)sizeof(float);
+        auto kern = gemm_stream_kernel<TO, TX, NW, RT, NT8, true, RELU2>;
+        constexpr int STATIC = (int)sizeof(float) * NW * SROWS * RT * (8 * NT8 + 1);
+        if (smem + STATIC > 48 * 1024) {
+            const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (err != cudaSuccess) return set_cuda_error(err);
+        }
+        kern<<<grid, NW * 32, smem, st>>>(p);
+    } else {
+        auto kern = p.K % 16 == 0 ? gemm_stream_kernel<TO, TX, NW, RT, NT8, true, RELU2>
+                                  : gemm_stream_kernel<TO, TX, NW, RT, NT8, false, RELU2>;
+        kern<<<grid, NW * 32, 0, st>>>(p);
+    }
     return check_launch();
 }
-
+// Measured with the weights out of L2 (e4m3 rows): 4096 x 1024 2.3 us with 8 warps; 4096 x 4096 7.5 us with 8,
+// 6.3 with 16; 8192 x 8192 17 with 8, 18 with 16; 64 groups of 2048 x 1024 with 36 in use 19.7 us with 8 warps, 15.5
+// = 4.9 TB/s with 4 warps and two tiles of W.
+template <typename TO, typename TX, bool RELU2>
+static int stream_launch(const GemmArgs& p, cudaStream_t st) {
+    const long long tiles = (long long)p.G * ((p.N + SROWS - 1) / SROWS);
+    if (tiles >= 2048) return stream_launch_t<TO, TX, 4, 2, 1, RELU2>(p, st);
+    if (p.K >= 2048 && tiles <= 296) return stream_launch_t<TO, TX, 16, 1, 1, RELU2>(p, st);
+    return stream_launch_t<TO, TX, 8, 1, 1, RELU2>(p, st);
+}
 int gemm_stream(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st) {
     if (epi == RELU2_Q) return RWKV_ERR_ARG;
+    if (p.x) {  // one group, plain product
+        RWKV_DISPATCH_DTYPE(out_dtype, T, return (stream_launch<T, T, false>(p, st)));
+        return RWKV_ERR_DTYPE;
+    }
     RWKV_DISPATCH_DTYPE(out_dtype, TO, {
-        return epi == RELU2 ? stream_launch<TO, true>(p, st) : stream_launch<TO, false>(p, st);
+        // 8 tokens a pass when a group has at most about that many rows, else 32
+        if ((long long)p.M > 8LL * p.G)
+            return epi == RELU2 ? stream_launch_t<TO, Quantised, 8, 1, 4, true>(p, st)
+                                : stream_launch_t<TO, Quantised, 8, 1, 4, false>(p, st);
+        return epi == RELU2 ? stream_launch<TO, Quantised, true>(p, st) : stream_launch<TO, Quantised, false>(p, st);
     });
     return RWKV_ERR_DTYPE;
 }
@@ -154,6 +255,14 @@ int gemm(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st) {
     return few ? fp8::gemm_stream(p, epi, out_dtype, st) : fp8::gemm_tc(p, epi, out_dtype, fp8::g_gemm_impl == 1 ? 0 : fp8::g_gemm_impl, st);
 }
 
+// Whether the streaming kernel can take a linear layer's x as it is and quantise it itself.  Not done
+// for the experts: their many CTAs would quantise the same rows over and over (64 rows, 64 experts of
+// 1024 x 2048: 40.6 us against 37 with two launches more).
+bool self_quantised(const void* x, long long ldx, int M, int K, int dtype) {
+    return fp8::g_gemm_impl <= 1 && M <= fp8::SELF_ROWS && K <= fp8::SELF_K && K % 16 == 0 && aligned(x, 16) &&
+           (ldx * (dtype == RWKV_F32 ? 4 : 2)) % 16 == 0;
+}
+
 }  // namespace
 
 extern "C" int rwkv_fp8_gemm(const void* a, long long lda, const float* a_scale, const void* w, long long ldw,
@@ -189,6 +298,10 @@ extern "C" int rwkv_fp8_linear(const void* x, long long ldx, const void* w, long
     if (!x || !out || !workspace) return RWKV_ERR_ARG;
     if (!aligned(workspace, 256)) return RWKV_ERR_ALIGN;
     if (workspace_bytes < rwkv_fp8_linear_workspace_size(M, K)) return RWKV_ERR_WORKSPACE;
+    if (self_quantised(x, ldx, M, K, dtype)) {
+        const GemmArgs p{nullptr, 0, nullptr, (const uint8_t*)w, ldw, 0, w_scale, nullptr, out, ldo, nullptr, M, N, K, 1, x, ldx};
+        return fp8::gemm_stream(p, fp8::STORE, dtype, (cudaStream_t)stream);
+    }
     uint8_t* q = (uint8_t*)workspace;
     float* qs = (float*)(q + rows_bytes(M, K));
     rc = rwkv_quantize_fp8_rows(x, ldx, q, pitch16(K), qs, M, K, dtype, stream);

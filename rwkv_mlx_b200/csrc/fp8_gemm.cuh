@@ -19,7 +19,13 @@ struct GemmArgs {
     long long ldo;
     float* os;          // RELU2_Q: (ceil(N / 128), M) scales of the output rows
     int M, N, K, G;
+    const void* x = nullptr;  // gemm_stream: rows of the output's type, still to be quantised, instead of a and as
+    long long ldx = 0;
 };
+
+// gemm_stream quantises x itself (in every CTA) for at most this many rows, K up to SELF_K, multiples
+// of 16, and 16-byte aligned rows.
+constexpr int SELF_ROWS = 8, SELF_K = 8192;
 
 int gemm_stream(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st);
 int gemm_tc(const GemmArgs& p, int epi, int out_dtype, int impl, cudaStream_t st);
