@@ -354,7 +354,8 @@ int rwkv_route_experts_backward(const void* logits, long long ld, const int32_t*
  *   (out_dtype unused; out_scale NULL otherwise).  Rows outside every group are not
  *   written.  M = 0 is valid.
  * rwkv_fp8_linear: out (M, N) = x w^T in dtype with x (M, K) in dtype quantised in the
- *   call, through a 256-byte aligned workspace of rwkv_fp8_linear_workspace_size bytes.
+ *   call, through a 256-byte aligned workspace of rwkv_fp8_linear_workspace_size bytes
+ *   (0 for few rows, which the product's own kernel quantises; workspace may then be NULL).
  * rwkv_fp8_experts: x (M, C) sorted by expert -> out (M, C) = the value product (val
  *   (E, C, D)) of the quantised relu(.)^2 of the key product (key (E, D, C)) of the
  *   quantised x, both in dtype; workspace 256-byte aligned. */

@@ -110,13 +110,20 @@ __global__ void __launch_bounds__(NW * 32) gemm_stream_kernel(const GemmArgs p) 
         if constexpr (SELF) {
             if (warp < nkb) load_w(warp);
             const int ntok = min(8, r1 - m0), l = lane & 15;
+            const bool xvec = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * sizeof(TX))) & 15) == 0;
             for (int b0 = 2 * warp; b0 < ntok * nkb; b0 += 2 * NW) {  // a block a half-warp
                 const int b = b0 + (lane >> 4), tok = b / nkb, kb = b % nkb, k = kb * BLK + l * 8;
                 const bool on = b < ntok * nkb;
                 float v[8], top = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[e] = 0.f;
-                if (on && k < p.K) load8(reinterpret_cast<const TX*>(p.x) + (long long)(m0 + tok) * p.ldx + k, v);
+                if (on && k < p.K) {
+                    const TX* x = reinterpret_cast<const TX*>(p.x) + (long long)(m0 + tok) * p.ldx + k;
+                    if (xvec) load8(x, v);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 8; e++) v[e] = to_f32(x[e]);
+                }
 #pragma unroll
                 for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(v[e]));
 #pragma unroll
@@ -255,12 +262,11 @@ int gemm(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st) {
     return few ? fp8::gemm_stream(p, epi, out_dtype, st) : fp8::gemm_tc(p, epi, out_dtype, fp8::g_gemm_impl == 1 ? 0 : fp8::g_gemm_impl, st);
 }
 
-// Whether the streaming kernel can take a linear layer's x as it is and quantise it itself.  Not done
+// Whether the streaming kernel takes a linear layer's x as it is and quantises it itself.  Not done
 // for the experts: their many CTAs would quantise the same rows over and over (64 rows, 64 experts of
 // 1024 x 2048: 40.6 us against 37 with two launches more).
-bool self_quantised(const void* x, long long ldx, int M, int K, int dtype) {
-    return fp8::g_gemm_impl <= 1 && M <= fp8::SELF_ROWS && K <= fp8::SELF_K && K % 16 == 0 && aligned(x, 16) &&
-           (ldx * (dtype == RWKV_F32 ? 4 : 2)) % 16 == 0;
+bool self_quantised(int M, int K) {
+    return fp8::g_gemm_impl <= 1 && M <= fp8::SELF_ROWS && K <= fp8::SELF_K && K % 16 == 0;
 }
 
 }  // namespace
@@ -284,7 +290,7 @@ extern "C" int rwkv_fp8_gemm(const void* a, long long lda, const float* a_scale,
 }
 
 extern "C" size_t rwkv_fp8_linear_workspace_size(int M, int K) {
-    return M <= 0 || K <= 0 ? 0 : rows_bytes(M, K) + scale_bytes(M, K);
+    return M <= 0 || K <= 0 || self_quantised(M, K) ? 0 : rows_bytes(M, K) + scale_bytes(M, K);
 }
 
 extern "C" int rwkv_fp8_linear(const void* x, long long ldx, const void* w, long long ldw, const float* w_scale,
@@ -295,13 +301,14 @@ extern "C" int rwkv_fp8_linear(const void* x, long long ldx, const void* w, long
     int rc = check_weight(w, ldw, 0, w_scale, 1, N, K);
     if (rc) return rc;
     if (M == 0) return RWKV_OK;
-    if (!x || !out || !workspace) return RWKV_ERR_ARG;
-    if (!aligned(workspace, 256)) return RWKV_ERR_ALIGN;
-    if (workspace_bytes < rwkv_fp8_linear_workspace_size(M, K)) return RWKV_ERR_WORKSPACE;
-    if (self_quantised(x, ldx, M, K, dtype)) {
+    if (!x || !out) return RWKV_ERR_ARG;
+    if (self_quantised(M, K)) {
         const GemmArgs p{nullptr, 0, nullptr, (const uint8_t*)w, ldw, 0, w_scale, nullptr, out, ldo, nullptr, M, N, K, 1, x, ldx};
         return fp8::gemm_stream(p, fp8::STORE, dtype, (cudaStream_t)stream);
     }
+    if (!workspace) return RWKV_ERR_ARG;
+    if (!aligned(workspace, 256)) return RWKV_ERR_ALIGN;
+    if (workspace_bytes < rwkv_fp8_linear_workspace_size(M, K)) return RWKV_ERR_WORKSPACE;
     uint8_t* q = (uint8_t*)workspace;
     float* qs = (float*)(q + rows_bytes(M, K));
     rc = rwkv_quantize_fp8_rows(x, ldx, q, pitch16(K), qs, M, K, dtype, stream);

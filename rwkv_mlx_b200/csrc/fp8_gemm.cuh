@@ -23,8 +23,8 @@ struct GemmArgs {
     long long ldx = 0;
 };
 
-// gemm_stream quantises x itself (in every CTA) for at most this many rows, K up to SELF_K, multiples
-// of 16, and 16-byte aligned rows.
+// gemm_stream quantises x itself (in every CTA) for at most this many rows and K up to SELF_K, a
+// multiple of 16.
 constexpr int SELF_ROWS = 8, SELF_K = 8192;
 
 int gemm_stream(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st);

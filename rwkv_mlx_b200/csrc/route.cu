@@ -22,7 +22,7 @@
 namespace rwkv {
 namespace route {
 
-constexpr int NT = 256, NW = NT / 32, MAXE = 512, MAXK = 32, MAXG = 32;
+constexpr int NT = 256, NW = NT / 32, CNT = 512 /* threads in a cluster's CTA */, MAXE = 512, MAXK = 32, MAXG = 32, MAXCLUSTER = 16;
 
 struct Args {
     const void* logits;
@@ -34,6 +34,7 @@ struct Args {
     int n, E, k, groups, keep, top2, renorm, sigmoid;
     int vec;  // rows 16-byte aligned
     float scale;
+    int cluster;  // the grid is one cluster: its CTAs add up their counters in shared memory
 };
 
 // Unsigned order of a float that an addition has produced (so NaN is the canonical positive one,
@@ -99,6 +100,19 @@ __device__ __forceinline__ void load_row(const T* row, int e0, int E, bool vec, 
     }
 }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The value at the same place of another CTA's shared memory.
+__device__ __forceinline__ uint32_t peer_value(const uint32_t* p, int rank) {
+    uint32_t a = (uint32_t)__cvta_generic_to_shared(p), v;
+    asm volatile("{ .reg .b32 ra; mapa.shared::cluster.u32 ra, %1, %2; ld.shared::cluster.u32 %0, [ra]; }"
+                 : "=r"(v)
+                 : "r"(a), "r"(rank)
+                 : "memory");
+    return v;
+}
+
 // Two largest of (a1 >= a2) and (b1 >= b2) as ordered keys.
 __device__ __forceinline__ void merge2(uint32_t& a1, uint32_t& a2, uint32_t b1, uint32_t b2) {
     a2 = max(min(a1, b1), max(a2, b2));
@@ -127,14 +141,14 @@ __device__ __forceinline__ void local2(const uint32_t (&key)[EPL], uint32_t gone
 enum Groups { ONE = 0, LANES = 1, ANY = 2 };
 
 template <typename T, int EPL, bool SIG, int GROUPS>
-__global__ void __launch_bounds__(NT, EPL <= 8 ? 4 : 2) route_kernel(const Args p) {
+__global__ void __launch_bounds__(CNT, EPL <= 8 ? 2 : 1) route_kernel(const Args p) {
     extern __shared__ uint32_t smem_route[];
     uint32_t* hist = smem_route;                                        // E counters (counts only)
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E, nw = blockDim.x >> 5;
     int* sel = reinterpret_cast<int*>(smem_route + (p.counts ? E : 0)) + warp * MAXK;   // this warp's choices
-    uint32_t* wkeys = smem_route + (p.counts ? E : 0) + NW * MAXK + warp * E;  // its keys (odd group sizes only)
+    uint32_t* wkeys = smem_route + (p.counts ? E : 0) + nw * MAXK + warp * E;  // its keys (odd group sizes only)
     if (p.counts) {
-        for (int e = threadIdx.x; e < E; e += NT) hist[e] = 0;
+        for (int e = threadIdx.x; e < E; e += blockDim.x) hist[e] = 0;
         __syncthreads();
     }
     const int e0 = lane * EPL, per = E / p.groups;
@@ -145,14 +159,14 @@ __global__ void __launch_bounds__(NT, EPL <= 8 ? 4 : 2) route_kernel(const Args 
     for (int i = 0; i < EPL; i++) b[i] = p.bias && e0 + i < E ? p.bias[e0 + i] : 0.f;
 
     float next[EPL];  // the next token's logits load during this token's selection
-    int t = blockIdx.x * NW + warp;
+    int t = blockIdx.x * nw + warp;
     if (t < p.n) load_row<T, EPL>(reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld, e0, E, p.vec, next);
-    for (; t < p.n; t += gridDim.x * NW) {
+    for (; t < p.n; t += gridDim.x * nw) {
         const T* row = reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld;
         float l[EPL];
 #pragma unroll
         for (int i = 0; i < EPL; i++) l[i] = next[i];
-        if (t + (int)gridDim.x * NW < p.n) load_row<T, EPL>(row + (long long)gridDim.x * NW * p.ld, e0, E, p.vec, next);
+        if (t + (int)gridDim.x * nw < p.n) load_row<T, EPL>(row + (long long)gridDim.x * nw * p.ld, e0, E, p.vec, next);
         float m = 0.f, z = 0.f;  // softmax: row maximum (0 for a row of -inf) and sum
         if (!SIG && (!by_logit || !p.renorm)) {
             m = -INFINITY;
@@ -257,10 +271,18 @@ __global__ void __launch_bounds__(NT, EPL <= 8 ? 4 : 2) route_kernel(const Args 
     }
     if (p.counts) {
         __syncthreads();
-        for (int e = threadIdx.x; e < E; e += NT) {
-            if (gridDim.x == 1) p.counts[e] = (int)hist[e];
+        if (p.cluster) cluster_sync();
+        for (int e = threadIdx.x; e < E; e += blockDim.x) {
+            if (p.cluster) {
+                if (blockIdx.x == 0) {
+                    uint32_t sum = 0;
+                    for (int r = 0; r < (int)gridDim.x; r++) sum += peer_value(&hist[e], r);
+                    p.counts[e] = (int)sum;
+                }
+            } else if (gridDim.x == 1) p.counts[e] = (int)hist[e];
             else if (hist[e]) atomicAdd(&p.counts[e], (int)hist[e]);  // integers: any order gives the same sum
         }
+        if (p.cluster) cluster_sync();  // the counters are read before their CTA leaves
     }
 }
 
@@ -353,17 +375,32 @@ static int grid_for(int n, int per_sm) {
 }
 
 template <typename T, int EPL>
-static void launch_fwd(const Args& p, int grid, cudaStream_t st) {
+static int launch_fwd(const Args& p, int grid, cudaStream_t st) {
     const int per = p.E / p.groups, lp = per / EPL;
     const int mode = p.groups == 1 ? ONE : per % EPL == 0 && (lp & (lp - 1)) == 0 ? LANES : ANY;
-    const size_t smem = sizeof(uint32_t) * (NW * MAXK + (p.counts ? p.E : 0) + (mode == ANY ? NW * p.E : 0));
+    const int nw = p.cluster ? CNT / 32 : NW;
+    const size_t smem = sizeof(uint32_t) * (nw * MAXK + (p.counts ? p.E : 0) + (mode == ANY ? nw * p.E : 0));
     auto kern = p.sigmoid ? (mode == ONE     ? route_kernel<T, EPL, true, ONE>
                              : mode == LANES ? route_kernel<T, EPL, true, LANES>
                                              : route_kernel<T, EPL, true, ANY>)
                           : (mode == ONE     ? route_kernel<T, EPL, false, ONE>
                              : mode == LANES ? route_kernel<T, EPL, false, LANES>
                                              : route_kernel<T, EPL, false, ANY>);
-    kern<<<grid, NT, smem, st>>>(p);
+    if (!p.cluster) {
+        kern<<<grid, NT, smem, st>>>(p);
+        return check_launch();
+    }
+    if (grid > 8) {
+        const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (err != cudaSuccess) return set_cuda_error(err);
+    }
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = grid, at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid), cfg.blockDim = dim3(CNT), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cfg.attrs = &at, cfg.numAttrs = 1;
+    return set_cuda_error(cudaLaunchKernelEx(&cfg, kern, p));
 }
 template <typename T, int EPL>
 static void launch_bwd(const BwdArgs& p, int grid, cudaStream_t st) {
@@ -394,18 +431,24 @@ extern "C" int rwkv_route_experts(const void* logits, long long ld, const float*
     if (n == 0) return counts ? set_cuda_error(cudaMemsetAsync(counts, 0, sizeof(int32_t) * E, st)) : RWKV_OK;
     if (!logits || !inds || !weights) return RWKV_ERR_ARG;
     const int es = dtype == RWKV_F32 ? 4 : 2;
-    route::Args p{logits, ld, bias, inds, weights, counts, n, E, k, groups, keep, group_top2, renormalize, sigmoid, 0, scale};
+    route::Args p{logits, ld, bias, inds, weights, counts, n, E, k, groups, keep, group_top2, renormalize, sigmoid, 0, scale, 0};
     p.vec = aligned(logits, 16) && (ld * es) % 16 == 0;
-    const int grid = route::grid_for(n, 8);
-    if (counts && grid > 1) {
+    int grid = route::grid_for(n, 8);
+    // With counts, up to 256 tokens run as one cluster, which needs no zeroed counters: 256 experts,
+    // 64 tokens 6.0 us instead of 8.3 with a memset before the kernel, 256 tokens 6.3 instead of 8.2.
+    constexpr int CW = route::CNT / 32;
+    if (counts && grid > 1 && n <= CW * route::MAXCLUSTER) {
+        p.cluster = 1;
+        grid = (n + CW - 1) / CW;
+    } else if (counts && grid > 1) {
         const int rc = set_cuda_error(cudaMemsetAsync(counts, 0, sizeof(int32_t) * E, st));
         if (rc) return rc;
     }
     RWKV_DISPATCH_DTYPE(dtype, T, {
-#define ROUTE_FWD(EPL) route::launch_fwd<T, EPL>(p, grid, st);
+#define ROUTE_FWD(EPL) return route::launch_fwd<T, EPL>(p, grid, st);
         ROUTE_BY_E(E, ROUTE_FWD)
     });
-    return check_launch();
+    return RWKV_ERR_DTYPE;
 }
 
 extern "C" int rwkv_route_experts_backward(const void* logits, long long ld, const int32_t* inds, const float* weights,

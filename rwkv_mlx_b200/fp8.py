@@ -26,9 +26,12 @@ def _blocks(n: int) -> int:
 
 
 def _empty_e4m3(rows: int, cols: int, dev) -> torch.Tensor:
-    pitch = -(-cols // 16) * 16
-    t = torch.empty((rows, pitch), device=dev, dtype=E4M3)
-    return t if pitch == cols else t[:, :cols]
+    return torch.empty_strided((rows, cols), (-(-cols // 16) * 16, 1), dtype=E4M3, device=dev)
+
+
+def _empty_scale(M: int, K: int, dev) -> torch.Tensor:
+    """(M, ceil(K / 128)) fp32, rows contiguous."""
+    return torch.empty_strided((M, _blocks(K)), (1, max(M, 1)), dtype=torch.float32, device=dev)
 
 
 def quantize_fp8_rows(x: torch.Tensor):
@@ -43,13 +46,13 @@ def quantize_fp8_rows(x: torch.Tensor):
     M, K = x.shape
     dev = x.device
     q = _empty_e4m3(M, K, dev)
-    scale = torch.empty((_blocks(K), M), device=dev, dtype=torch.float32)
+    scale = _empty_scale(M, K, dev)
     L = nat.lib()
     with nat.on_device(dev):
-        rc = L.rwkv_quantize_fp8_rows(nat.ptr(x), nat.row_stride(x), nat.ptr(q), q.stride(0), nat.ptr(scale), M, K, code,
-                                      nat.stream_ptr(dev))
+        rc = L.rwkv_quantize_fp8_rows(x.data_ptr(), nat.row_stride(x), q.data_ptr(), q.stride(0), scale.data_ptr(), M, K,
+                                      code, nat.stream_ptr(dev))
     nat.check(rc, "rwkv_quantize_fp8_rows")
-    return q, scale.t()
+    return q, scale
 
 
 def quantize_fp8_weight(w: torch.Tensor):
@@ -160,9 +163,9 @@ def fp8_matmul_relu_sq_quantized(a: torch.Tensor, a_scale: torch.Tensor, w: torc
     rows of a squared-ReLU layer): returns (q (M, N) e4m3, scale (M, ceil(N / 128)))."""
     M, N, dev = a.shape[0], w.shape[-2], a.device
     q = _empty_e4m3(M, N, dev)
-    scale = torch.empty((_blocks(N), M), device=dev, dtype=torch.float32)
+    scale = _empty_scale(M, N, dev)
     _gemm("fp8_matmul_relu_sq_quantized", a, a_scale, w, w_scale, offsets, q, scale, 2, 0)
-    return q, scale.t()
+    return q, scale
 
 
 def _linear(x2d, w, w_scale):
@@ -175,13 +178,13 @@ def _linear(x2d, w, w_scale):
                          "(ceil(N / 128), ceil(K / 128)) on x's device")
     N = w.shape[0]
     code = nat.dtype_code(x2d)
-    out = torch.empty((M, N), device=dev, dtype=x2d.dtype)
+    out = torch.empty_strided((M, N), (N, 1), dtype=x2d.dtype, device=dev)
     L = nat.lib()
     nws = L.rwkv_fp8_linear_workspace_size(M, K)
-    ws = torch.empty(nws, device=dev, dtype=torch.uint8)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
     with nat.on_device(dev):
         rc = L.rwkv_fp8_linear(x2d.data_ptr(), nat.row_stride(x2d), w.data_ptr(), nat.row_stride(w),
-                               w_scale.contiguous().data_ptr(), out.data_ptr(), N, ws.data_ptr(), nws, M, N, K, code,
+                               w_scale.contiguous().data_ptr(), out.data_ptr(), N, nat.ptr(ws), nws, M, N, K, code,
                                nat.stream_ptr(dev))
     nat.check(rc, "rwkv_fp8_linear")
     return out

@@ -20,9 +20,10 @@ MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 512, 32, 32
 def _forward(logits, top_k, sigmoid, bias, n_groups, topk_groups, top2, renormalize, scale, want_counts):
     n, E = logits.shape
     dev = logits.device
-    inds = torch.empty((n, top_k), device=dev, dtype=torch.int32)
-    weights = torch.empty((n, top_k), device=dev, dtype=torch.float32)
-    counts = torch.empty(E, device=dev, dtype=torch.int32) if want_counts else None
+    shape, pitch = (n, top_k), (top_k, 1)  # (empty_strided costs less than empty on the host)
+    inds = torch.empty_strided(shape, pitch, dtype=torch.int32, device=dev)
+    weights = torch.empty_strided(shape, pitch, dtype=torch.float32, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev) if want_counts else None
     L = nat.lib()
     with nat.on_device(dev):
         rc = L.rwkv_route_experts(nat.ptr(logits), nat.row_stride(logits), nat.ptr(bias), nat.ptr(inds),
