@@ -17,41 +17,56 @@ constexpr int QT = 128, QROWS = QT / 16, QU = 4;  // threads, rows of a CTA, blo
 // VEC: rows are 16-byte aligned and K is a multiple of 8, so a lane's 8 values are all in the
 // row or all past it.  The loads then stay raw until all of them are on their way (converting
 // inside the guarded load made each wait for the one before: 33 against 19 us at 32768 x 1024).
-template <typename T, bool VEC>
+// GRAD: the gradient through h = relu(u)^2 on the way in, x 2 relu(u) with u in x's layout, formed in
+// fp32 and never stored (x and u: the same type).
+template <typename T, bool VEC, bool GRAD>
 __global__ void __launch_bounds__(QT)
-    quant_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q, long long ldq,
-                      float* __restrict__ scale, int M, int K) {
+    quant_rows_kernel(const T* __restrict__ x, const T* __restrict__ u, long long ldx, uint8_t* __restrict__ q,
+                      long long ldq, float* __restrict__ scale, int M, int K) {
     constexpr int NV = sizeof(T) / 2;  // 16-byte loads for 8 values
     const int row = blockIdx.x * QROWS + (threadIdx.x >> 4), l = threadIdx.x & 15;
     const int kb0 = blockIdx.y * QU;
     const bool on = row < M;
-    const T* xr = x + (long long)row * ldx;
+    const T *xr = x + (long long)row * ldx, *ur = GRAD ? u + (long long)row * ldx : nullptr;
     uint8_t* qr = q + (long long)row * ldq;
     __shared__ float sm[QU][QROWS];
-    uint4 raw[QU][NV];
+    uint4 raw[QU][NV], rawu[GRAD ? QU : 1][NV];
 #pragma unroll
-    for (int u = 0; u < QU; u++) {
-        const int k = (kb0 + u) * BLK + l * 8;
+    for (int b = 0; b < QU; b++) {
+        const int k = (kb0 + b) * BLK + l * 8;
 #pragma unroll
-        for (int i = 0; i < NV; i++) raw[u][i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < NV; i++) {
+            raw[b][i] = make_uint4(0u, 0u, 0u, 0u);
+            if (GRAD) rawu[b][i] = make_uint4(0u, 0u, 0u, 0u);
+        }
         if (VEC) {
             if (on && k < K) {
 #pragma unroll
-                for (int i = 0; i < NV; i++) raw[u][i] = __ldg(reinterpret_cast<const uint4*>(xr + k) + i);
+                for (int i = 0; i < NV; i++) {
+                    raw[b][i] = __ldg(reinterpret_cast<const uint4*>(xr + k) + i);
+                    if (GRAD) rawu[b][i] = __ldg(reinterpret_cast<const uint4*>(ur + k) + i);
+                }
             }
         } else {
-            T* r = reinterpret_cast<T*>(raw[u]);
+            T *r = reinterpret_cast<T*>(raw[b]), *ru = reinterpret_cast<T*>(rawu[GRAD ? b : 0]);
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if (on && k + e < K) r[e] = xr[k + e];
+                if (on && k + e < K) {
+                    r[e] = xr[k + e];
+                    if (GRAD) ru[e] = ur[k + e];
+                }
         }
     }
 #pragma unroll
-    for (int u = 0; u < QU; u++) {
-        const T* r = reinterpret_cast<const T*>(raw[u]);
+    for (int b = 0; b < QU; b++) {
+        const T* r = reinterpret_cast<const T*>(raw[b]);
         float v[8], a = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = to_f32(r[e]), a = fmaxf(a, fabsf(v[e]));
+        for (int e = 0; e < 8; e++) {
+            v[e] = to_f32(r[e]);
+            if (GRAD) v[e] *= 2.f * relu(to_f32(reinterpret_cast<const T*>(rawu[GRAD ? b : 0])[e]));
+            a = fmaxf(a, fabsf(v[e]));
+        }
 #pragma unroll
         for (int o = 8; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
         a = clamp_amax(a);
@@ -59,18 +74,18 @@ __global__ void __launch_bounds__(QT)
         uint2 w;
         w.x = pack4(v[0] * mul, v[1] * mul, v[2] * mul, v[3] * mul);
         w.y = pack4(v[4] * mul, v[5] * mul, v[6] * mul, v[7] * mul);
-        const int k = (kb0 + u) * BLK + l * 8;
+        const int k = (kb0 + b) * BLK + l * 8;
         if (on && k < K) {
             if (VEC || k + 8 <= K) {
                 *reinterpret_cast<uint2*>(qr + k) = w;
             } else {
-                const uint8_t* b = reinterpret_cast<const uint8_t*>(&w);
+                const uint8_t* by = reinterpret_cast<const uint8_t*>(&w);
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                    if (k + e < K) qr[k + e] = b[e];
+                    if (k + e < K) qr[k + e] = by[e];
             }
         }
-        if (l == 0) sm[u][threadIdx.x >> 4] = dequant_scale(a);
+        if (l == 0) sm[b][threadIdx.x >> 4] = dequant_scale(a);
     }
     // the rows' scales of a block leave together: one by one they cost 2 of 20 us
     __syncthreads();
@@ -80,19 +95,39 @@ __global__ void __launch_bounds__(QT)
     }
 }
 
-// One CTA per 128 x 128 block; each thread keeps 64 values (half a row of the block).
-template <typename T>
+// One CTA per 128 x 128 block: 16 lanes a row, 8 rows a thread, all loads on their way before the
+// block's maximum is formed; the raw values stay in registers.  VEC as above.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     quant_weight_kernel(const T* __restrict__ w, uint8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
                         int N, int K) {
+    constexpr int NV = sizeof(T) / 2, R = 8;
     const int kb = blockIdx.x, nb = blockIdx.y, g = blockIdx.z;
-    const int n = nb * BLK + (threadIdx.x >> 1), k0 = kb * BLK + (threadIdx.x & 1) * 64;
-    const T* wr = w + ((long long)g * N + n) * K;
-    uint8_t* qr = q + ((long long)g * N + n) * ldq;
+    const int k = kb * BLK + (threadIdx.x & 15) * 8, n0 = nb * BLK + (threadIdx.x >> 4);
+    uint4 raw[R][NV];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int n = n0 + 16 * r;
+        const T* wr = w + ((long long)g * N + n) * K + k;
+#pragma unroll
+        for (int i = 0; i < NV; i++) raw[r][i] = make_uint4(0u, 0u, 0u, 0u);
+        if (VEC) {
+            if (n < N && k < K) {
+#pragma unroll
+                for (int i = 0; i < NV; i++) raw[r][i] = __ldg(reinterpret_cast<const uint4*>(wr) + i);
+            }
+        } else {
+            T* t = reinterpret_cast<T*>(raw[r]);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (n < N && k + e < K) t[e] = wr[e];
+        }
+    }
     float a = 0.f;
-    if (n < N)
-        for (int e = 0; e < 64; e++)
-            if (k0 + e < K) a = fmaxf(a, fabsf(to_f32(wr[k0 + e])));
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) a = fmaxf(a, fabsf(to_f32(reinterpret_cast<const T*>(raw[r])[e])));
     __shared__ float part[8];
 #pragma unroll
     for (int o = 16; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
@@ -102,14 +137,26 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < 8; i++) a = fmaxf(a, part[i]);
     a = clamp_amax(a);
     const float mul = quant_mul(a);
-    if (n < N)
-        for (int e = 0; e < 64; e += 2) {
-            if (k0 + e + 1 < K)
-                *reinterpret_cast<uint16_t*>(qr + k0 + e) =
-                    (uint16_t)pack2(to_f32(wr[k0 + e]) * mul, to_f32(wr[k0 + e + 1]) * mul);
-            else if (k0 + e < K)
-                qr[k0 + e] = (uint8_t)pack2(to_f32(wr[k0 + e]) * mul, 0.f);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int n = n0 + 16 * r;
+        if (n >= N || k >= K) continue;
+        uint8_t* qr = q + ((long long)g * N + n) * ldq + k;
+        const T* t = reinterpret_cast<const T*>(raw[r]);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = to_f32(t[e]) * mul;
+        uint2 b;
+        b.x = pack4(v[0], v[1], v[2], v[3]), b.y = pack4(v[4], v[5], v[6], v[7]);
+        if (VEC || k + 8 <= K) {
+            *reinterpret_cast<uint2*>(qr) = b;
+        } else {
+            const uint8_t* p = reinterpret_cast<const uint8_t*>(&b);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (k + e < K) qr[e] = p[e];
         }
+    }
     if (threadIdx.x == 0) scale[((long long)g * gridDim.y + nb) * gridDim.x + kb] = dequant_scale(a);
 }
 
@@ -118,23 +165,35 @@ __global__ void __launch_bounds__(256)
 
 using namespace rwkv;
 
-extern "C" int rwkv_quantize_fp8_rows(const void* x, long long ldx, void* q, long long ldq, float* scale, int M, int K,
-                                      int dtype, void* stream) {
+static int quantize_rows(const void* x, const void* u, long long ldx, void* q, long long ldq, float* scale, int M, int K,
+                         int dtype, void* stream) {
     if (dtype != RWKV_F32 && dtype != RWKV_F16 && dtype != RWKV_BF16) return RWKV_ERR_DTYPE;
     if (M < 0 || K <= 0 || ldx < K || ldq < K) return RWKV_ERR_SHAPE;
     if (M == 0) return RWKV_OK;
     if (!x || !q || !scale) return RWKV_ERR_ARG;
     if (!aligned(q, 8) || ldq % 8) return RWKV_ERR_ALIGN;
     const int es = dtype == RWKV_F32 ? 4 : 2;
-    const bool vec = aligned(x, 16) && (ldx * es) % 16 == 0 && K % 8 == 0;
+    const bool vec = aligned(x, 16) && aligned(u, 16) && (ldx * es) % 16 == 0 && K % 8 == 0;
     const int nkb = (K + fp8::BLK - 1) / fp8::BLK;
     const dim3 grid((M + fp8::QROWS - 1) / fp8::QROWS, (nkb + fp8::QU - 1) / fp8::QU);
     if (grid.y > 65535) return RWKV_ERR_SHAPE;
     RWKV_DISPATCH_DTYPE(dtype, T, {
-        auto kern = vec ? fp8::quant_rows_kernel<T, true> : fp8::quant_rows_kernel<T, false>;
-        kern<<<grid, fp8::QT, 0, (cudaStream_t)stream>>>((const T*)x, ldx, (uint8_t*)q, ldq, scale, M, K);
+        auto kern = u ? (vec ? fp8::quant_rows_kernel<T, true, true> : fp8::quant_rows_kernel<T, false, true>)
+                      : (vec ? fp8::quant_rows_kernel<T, true, false> : fp8::quant_rows_kernel<T, false, false>);
+        kern<<<grid, fp8::QT, 0, (cudaStream_t)stream>>>((const T*)x, (const T*)u, ldx, (uint8_t*)q, ldq, scale, M, K);
     });
     return check_launch();
+}
+
+extern "C" int rwkv_quantize_fp8_rows(const void* x, long long ldx, void* q, long long ldq, float* scale, int M, int K,
+                                      int dtype, void* stream) {
+    return quantize_rows(x, nullptr, ldx, q, ldq, scale, M, K, dtype, stream);
+}
+
+extern "C" int rwkv_quantize_fp8_relu_sq_grad(const void* dh, const void* u, long long ld, void* q, long long ldq,
+                                              float* scale, int M, int K, int dtype, void* stream) {
+    if (M > 0 && !u) return RWKV_ERR_ARG;
+    return quantize_rows(dh, u, ld, q, ldq, scale, M, K, dtype, stream);
 }
 
 extern "C" int rwkv_quantize_fp8_weight(const void* w, void* q, long long ldq, float* scale, int G, int N, int K,
@@ -146,8 +205,8 @@ extern "C" int rwkv_quantize_fp8_weight(const void* w, void* q, long long ldq, f
     const dim3 grid((K + fp8::BLK - 1) / fp8::BLK, (N + fp8::BLK - 1) / fp8::BLK, G);
     if (grid.y > 65535 || grid.z > 65535) return RWKV_ERR_SHAPE;
     RWKV_DISPATCH_DTYPE(dtype, T, {
-        fp8::quant_weight_kernel<T>
-            <<<grid, 256, 0, (cudaStream_t)stream>>>((const T*)w, (uint8_t*)q, ldq, scale, N, K);
+        auto kern = aligned(w, 16) && K % 8 == 0 ? fp8::quant_weight_kernel<T, true> : fp8::quant_weight_kernel<T, false>;
+        kern<<<grid, 256, 0, (cudaStream_t)stream>>>((const T*)w, (uint8_t*)q, ldq, scale, N, K);
     });
     return check_launch();
 }

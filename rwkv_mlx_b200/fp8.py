@@ -14,6 +14,7 @@ the rows contiguous, weight scales (..., ceil(N / 128), ceil(K / 128)) fp32 cont
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -197,6 +198,7 @@ class _Linear(torch.autograd.Function):
         return _linear(x2d, w, w_scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         return _linear(nat.rows_2d(dy), *ctx.saved_tensors), None, None, None, None
 
@@ -223,32 +225,68 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, w_t: tor
     return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
 
 
+def _experts(x, key, key_scale, value, value_scale, offsets, C, D, E, ldk, ldv):
+    M, dev = x.shape[0], x.device
+    out = torch.empty_strided((M, C), (C, 1), dtype=x.dtype, device=dev)
+    L = nat.lib()
+    nws = L.rwkv_fp8_experts_workspace_size(M, C, D, E)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+    with nat.on_device(dev):
+        rc = L.rwkv_fp8_experts(x.data_ptr(), nat.row_stride(x), key.data_ptr(), ldk, key.stride(0), key_scale.data_ptr(),
+                                value.data_ptr(), ldv, value.stride(0), value_scale.data_ptr(), nat.ptr(offsets),
+                                out.data_ptr(), C, ws.data_ptr(), nws, M, C, D, E, nat.dtype_code(x), nat.stream_ptr(dev))
+    nat.check(rc, "rwkv_fp8_experts")
+    return out
+
+
+class _Experts(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weights, transposed, offsets, dims):
+        ctx.save_for_backward(x, offsets, *weights[:2], *transposed)
+        return _experts(x, *weights, offsets, *dims)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, offsets, key, key_scale, key_t, key_t_scale, value_t, value_t_scale = ctx.saved_tensors
+        # u again rather than kept from the forward pass (there it never leaves the key product's kernel)
+        u = fp8_matmul(*quantize_fp8_rows(x), key, key_scale, offsets, out_dtype=x.dtype)
+        dh = fp8_matmul(*quantize_fp8_rows(dy), value_t, value_t_scale, offsets, out_dtype=x.dtype)
+        M, D = u.shape
+        q, scale = _empty_e4m3(M, D, x.device), _empty_scale(M, D, x.device)
+        L = nat.lib()
+        with nat.on_device(x.device):
+            rc = L.rwkv_quantize_fp8_relu_sq_grad(dh.data_ptr(), u.data_ptr(), D, q.data_ptr(), q.stride(0),
+                                                  scale.data_ptr(), M, D, nat.dtype_code(u), nat.stream_ptr(x.device))
+        nat.check(rc, "rwkv_quantize_fp8_relu_sq_grad")
+        return fp8_matmul(q, scale, key_t, key_t_scale, offsets, out_dtype=x.dtype), None, None, None, None
+
+
 def fp8_experts(rows: torch.Tensor, key: torch.Tensor, key_scale: torch.Tensor, value: torch.Tensor,
-                value_scale: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+                value_scale: torch.Tensor, offsets: torch.Tensor, transposed: tuple | None = None) -> torch.Tensor:
     """Each expert's squared-ReLU layer over its rows: value_e(q(relu(key_e(q(x)))^2)), in rows' dtype.
 
     rows (M, C) sorted by expert, expert e owning [offsets[e], offsets[e + 1]); key (E, D, C) and
-    value (E, C, D) e4m3 with their scales.  Rows outside every expert are undefined.  Forward only."""
-    if torch.is_grad_enabled() and rows.requires_grad:
-        raise RuntimeError("fp8_experts: forward only; call it under torch.no_grad() or on rows without gradient")
+    value (E, C, D) e4m3 with their scales.  Rows outside every expert are undefined.
+
+    The weights are frozen.  For rows that require grad, pass ``transposed`` = (key_t, key_t_scale,
+    value_t, value_t_scale), the two weights through :func:`transpose_fp8_weight`: with u = q(x) key^T,
+    dx = q(q(dy) value * 2 relu(u)) key, the quantisations' own derivatives taken as 1."""
     if rows.dim() != 2 or key.dim() != 3 or value.dim() != 3 or value.shape != (key.shape[0], key.shape[2], key.shape[1]) \
             or key.shape[2] != rows.shape[1]:
         raise ValueError(f"fp8_experts: rows {tuple(rows.shape)}, key {tuple(key.shape)} and value {tuple(value.shape)} "
                          "do not fit (key (E, D, C), value (E, C, D))")
-    code = nat.dtype_code(rows)
+    nat.dtype_code(rows)
     x = nat.rows_2d(rows)
-    M, C = x.shape
-    dev = x.device
+    C, dev = x.shape[1], x.device
     key, key_scale, E, D, ldk = _check_weight("fp8_experts", key, key_scale, C, dev)
     value, value_scale, _, _, ldv = _check_weight("fp8_experts", value, value_scale, D, dev)
     _check_offsets("fp8_experts", offsets, E, dev)
-    out = torch.empty((M, C), device=dev, dtype=x.dtype)
-    L = nat.lib()
-    nws = L.rwkv_fp8_experts_workspace_size(M, C, D, E)
-    ws = torch.empty(nws, device=dev, dtype=torch.uint8)
-    with nat.on_device(dev):
-        rc = L.rwkv_fp8_experts(x.data_ptr(), nat.row_stride(x), key.data_ptr(), ldk, key.stride(0), key_scale.data_ptr(),
-                                value.data_ptr(), ldv, value.stride(0), value_scale.data_ptr(), nat.ptr(offsets),
-                                out.data_ptr(), C, ws.data_ptr(), nws, M, C, D, E, code, nat.stream_ptr(dev))
-    nat.check(rc, "rwkv_fp8_experts")
-    return out
+    if rows.requires_grad and torch.is_grad_enabled():
+        if transposed is None:
+            raise RuntimeError("fp8_experts: rows that require grad need the transposed weights for the gradient")
+        key_t, value_t = transposed[0], transposed[2]
+        if key_t.shape != (E, C, D) or value_t.shape != (E, D, C):
+            raise ValueError("fp8_experts: transposed must be key (E, C, D) and value (E, D, C) with their scales")
+        return _Experts.apply(x, (key, key_scale, value, value_scale), transposed, offsets, (C, D, E, ldk, ldv))
+    return _experts(x, key, key_scale, value, value_scale, offsets, C, D, E, ldk, ldv)

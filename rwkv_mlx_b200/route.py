@@ -11,6 +11,7 @@ reference.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -45,6 +46,7 @@ class _Route(torch.autograd.Function):
         return inds, weights, counts
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, _dinds, dweights, _dcounts=None):
         if dweights is None:
             return (None,) * 10

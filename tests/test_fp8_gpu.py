@@ -306,6 +306,78 @@ def test_experts_match_their_parts(M, E, dtype):
     assert rel_rms(y.double().cpu().numpy(), ref.double().cpu().numpy()) < 1e-3 + 2 * ULP[dtype]
 
 
+@pytest.mark.parametrize("M,E", [(7, 4), (700, 3)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_experts_gradient(M, E, dtype):
+    """dx against the formula in float64 with the quantisations where the operator has them (q(dy), q(du); u and dh are
+    rounded to the rows' type on the way: an ulp each, and a few of q(du)'s values on the other side of a
+    step of 2^-4: 2^-4 * sqrt(2 ulp)), and against the float64 layer's own gradient, from which the
+    quantised dy, du and hidden rows differ by 2^-5 or so each."""
+    from rwkv_mlx_b200.fp8 import fp8_experts, quantize_fp8_weight, transpose_fp8_weight
+
+    C, D = 136, 264
+    g = gen(M)
+    key, ks = quantize_fp8_weight(torch.randn(E, D, C, device="cuda", generator=g) / 12)
+    val, vs = quantize_fp8_weight(torch.randn(E, C, D, device="cuda", generator=g) / 16)
+    tr = (*transpose_fp8_weight(key, ks), *transpose_fp8_weight(val, vs))
+    sizes = torch.bincount(torch.randint(1, E, (M,), device="cuda", generator=g), minlength=E)
+    offs = torch.cat([sizes.new_zeros(1), sizes.cumsum(0)]).int()
+    x = torch.randn(M, C, device="cuda", generator=g).to(dtype).requires_grad_(True)
+    y = fp8_experts(x, key, ks, val, vs, offs, tr)
+    with torch.no_grad():
+        assert torch.equal(y, fp8_experts(x, key, ks, val, vs, offs))
+    dy = torch.randn(M, C, device="cuda", generator=g).to(dtype)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    K, V = weight64(key, ks), weight64(val, vs)
+    xq, dyq = rows64(*plain_rows(x.detach())), rows64(*plain_rows(dy))
+    ref, free = torch.zeros(M, C, dtype=torch.float64), torch.zeros(M, C, dtype=torch.float64)
+    for e in range(E):
+        lo, hi = int(offs[e]), int(offs[e + 1])
+        u = (xq[lo:hi] @ K[e].T).to(dtype).double()
+        dh = (dyq[lo:hi] @ V[e]).to(dtype).double()
+        du = dh * 2 * u.clamp(min=0)
+        if hi > lo:
+            ref[lo:hi] = rows64(*plain_rows(du)) @ K[e]
+        xe = x[lo:hi].detach().cpu().double().requires_grad_(True)
+        ((xe @ K[e].T).clamp(min=0) ** 2 @ V[e].T).backward(dy[lo:hi].cpu().double())
+        free[lo:hi] = xe.grad
+    ulp = max(ULP[dtype], 2.0 ** -20)
+    assert dx.dtype == dtype
+    assert rel_rms(dx.cpu().double().numpy(), ref.numpy()) < 4 * ulp + 2.0 ** -4 * math.sqrt(2 * ulp)
+    assert rel_rms(dx.cpu().double().numpy(), free.numpy()) < 0.08
+
+
+@pytest.mark.parametrize("M,K", [(3, 127), (130, 776), (33, 1024)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_relu_sq_grad_bytes(dtype, M, K):
+    from rwkv_mlx_b200 import _native as nat
+
+    dh, u = data(M, K, 1, dtype), data(M, K, 2, dtype)
+    q = torch.zeros(M, -(-K // 16) * 16, device="cuda", dtype=torch.uint8)
+    s = torch.zeros(blocks(K), M, device="cuda")
+    nat.check(nat.lib().rwkv_quantize_fp8_relu_sq_grad(dh.data_ptr(), u.data_ptr(), K, q.data_ptr(), q.stride(0),
+                                                       s.data_ptr(), M, K, nat.dtype_code(dh), nat.stream_ptr(dh.device)),
+              "rwkv_quantize_fp8_relu_sq_grad")
+    qr, sr = plain_rows(dh.float().cpu() * (2 * u.float().cpu().clamp(min=0)))
+    assert torch.equal(q[:, :K].cpu(), qr.view(torch.uint8)) and torch.equal(s.t().cpu(), sr)
+
+
+def test_second_derivatives_are_refused():
+    """The backward passes are not differentiable themselves: asking for that raises instead of leaving terms out."""
+    from rwkv_mlx_b200.fp8 import fp8_linear, quantize_fp8_weight, transpose_fp8_weight
+    from rwkv_mlx_b200.route import route_experts
+
+    w = quantize_fp8_weight(torch.randn(64, 32, device="cuda"))
+    x = torch.randn(3, 32, device="cuda", requires_grad=True)
+    c = torch.randn(3, 64, device="cuda", requires_grad=True)
+    (d,) = torch.autograd.grad((fp8_linear(x, *w, *transpose_fp8_weight(*w)) * c).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
+    (d,) = torch.autograd.grad(route_experts(x, 4)[1].square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
+
+
 def test_offsets_past_32_bits():
     """Rows whose byte offset exceeds 2^32 in the activations, the e4m3 rows and the outputs."""
     from rwkv_mlx_b200.fp8 import fp8_linear, quantize_fp8_weight
@@ -419,6 +491,8 @@ def test_refusals():
     vq, vs = quantize_fp8_weight(torch.randn(2, 256, 128, device="cuda"))
     with pytest.raises(RuntimeError):
         fp8_experts(x.float().requires_grad_(True), wq, ws, vq, vs, offs)
+    with pytest.raises(ValueError):
+        fp8_experts(x.float().requires_grad_(True), wq, ws, vq, vs, offs, (wq, ws, vq, vs))
 
 
 @pytest.mark.parametrize("own_router", [True, False])
