@@ -13,10 +13,15 @@
 // One warp per token.  Lane i holds the EPL consecutive experts from i * EPL on, so the
 // lowest lane of a tie also has the lowest expert, and a group is a run of lanes when EPL
 // divides its size.  Keys are compared as unsigned integers that order like the floats: a
-// round of the top-k is one redux.sync over the lanes' best keys, a ballot and a rescan of
-// the winner's EPL keys.  expf and the reciprocal are CUDA's correctly rounded or
+// round of the top-k is one redux.sync over the lanes' best keys and a ballot, after which the
+// winner moves on to its next key.  expf and the reciprocal are CUDA's correctly rounded or
 // few-ulp functions, not the fast forms, so that keys agree with the formula evaluated in
 // fp32 elsewhere and no near-tie flips.
+//
+// Bound by instruction issue, not by its 4 E bytes a token: about 900 warp instructions a token
+// of 256 experts in 8 groups (scores 140, the lanes' best three 110, groups 160, 40 a choice),
+// 36 us for 32768 tokens where the traffic alone would take 5.5; the gradient writes E values
+// a token and is bound by that (16381 x 96 in bf16: 3.9 us).
 #include "common.cuh"
 
 namespace rwkv {
@@ -122,19 +127,50 @@ __device__ __forceinline__ float unkey(uint32_t u) {
     return __uint_as_float(u ^ ((uint32_t)((int)~u >> 31) | 0x80000000u));
 }
 
-// The lane's two largest keys outside `gone` and their positions (ties: the lower position first).
+// The lane's three largest keys and their positions (ties: the lower position first) among those that
+// come after the key `last` at position `li` in that order; last = ~0, li = -1: all.
+struct Best {
+    uint32_t k1, k2, k3;
+    int i1, i2, i3;
+};
 template <int EPL>
-__device__ __forceinline__ void local2(const uint32_t (&key)[EPL], uint32_t gone, uint32_t& k1, int& i1, uint32_t& k2, int& i2) {
-    k1 = k2 = 0u, i1 = i2 = 0;
+__device__ __forceinline__ Best local3(const uint32_t (&key)[EPL], uint32_t last, int li) {
+    Best b{0u, 0u, 0u, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < EPL; i++) {
-        const uint32_t k = (gone >> i) & 1u ? 0u : key[i];
-        const bool p1 = k > k1, p2 = k > k2;
-        i2 = p1 ? i1 : (p2 ? i : i2);
-        i1 = p1 ? i : i1;
-        k2 = max(k2, min(k1, k));
-        k1 = max(k1, k);
+        const uint32_t k = key[i] < last || (key[i] == last && i > li) ? key[i] : 0u;
+        const bool p1 = k > b.k1, p2 = k > b.k2, p3 = k > b.k3;
+        b.i3 = p2 ? b.i2 : (p3 ? i : b.i3);
+        b.k3 = max(b.k3, min(b.k2, k));
+        b.i2 = p1 ? b.i1 : (p2 ? i : b.i2);
+        b.k2 = max(b.k2, min(b.k1, k));
+        b.i1 = p1 ? i : b.i1;
+        b.k1 = max(b.k1, k);
     }
+    return b;
+}
+
+// The k largest keys of the warp in order: lane j returns the j-th one's expert.  b: the lane's best
+// three; few tokens take more than three from a lane, which then looks for the next ones.
+template <int EPL>
+__device__ __forceinline__ int top_k(const uint32_t (&key)[EPL], Best b, int k, int e0, int lane) {
+    const uint32_t below = (1u << lane) - 1;
+    int choice = 0;
+    for (int j = 0; j < k; j++) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, b.k1);
+        const uint32_t tied = __ballot_sync(0xffffffffu, b.k1 == top);
+        const int pos = b.i1, e = __shfl_sync(0xffffffffu, e0 + pos, __ffs(tied) - 1);
+        if (lane == j) choice = e;
+        bool again = false;
+        if (b.k1 == top && !(tied & below)) {  // of tied lanes the lowest
+            again = EPL > 3 && b.k2 == 0u;
+            b.k1 = b.k2, b.i1 = b.i2;
+            b.k2 = b.k3, b.i2 = b.i3;
+            b.k3 = 0u;
+        }
+        if (again) b = local3<EPL>(key, top, pos);
+    }
+    return choice;
 }
 
 // Groups: none, runs of lanes (their size a power of two times EPL), or any equal runs.
@@ -145,18 +181,19 @@ __global__ void __launch_bounds__(CNT, EPL <= 8 ? 2 : 1) route_kernel(const Args
     extern __shared__ uint32_t smem_route[];
     uint32_t* hist = smem_route;                                        // E counters (counts only)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E, nw = blockDim.x >> 5;
-    int* sel = reinterpret_cast<int*>(smem_route + (p.counts ? E : 0)) + warp * MAXK;   // this warp's choices
-    uint32_t* wkeys = smem_route + (p.counts ? E : 0) + nw * MAXK + warp * E;  // its keys (odd group sizes only)
+    uint32_t* wkeys = smem_route + (p.counts ? E : 0) + warp * E;  // this warp's keys (odd group sizes only)
     if (p.counts) {
         for (int e = threadIdx.x; e < E; e += blockDim.x) hist[e] = 0;
         __syncthreads();
     }
     const int e0 = lane * EPL, per = E / p.groups;
     const int lanes_per = per / EPL;  // LANES: lanes of a group
+    const int lp_log = GROUPS == LANES ? __ffs(lanes_per) - 1 : 0;
     const bool by_logit = !SIG && !p.bias && !(GROUPS != ONE && p.top2);
     float b[EPL];
 #pragma unroll
-    for (int i = 0; i < EPL; i++) b[i] = p.bias && e0 + i < E ? p.bias[e0 + i] : 0.f;
+    // positions past E get -inf, so their keys rank below or tie with every expert's, which have the lower index
+    for (int i = 0; i < EPL; i++) b[i] = e0 + i >= E ? -INFINITY : p.bias ? p.bias[e0 + i] : 0.f;
 
     float next[EPL];  // the next token's logits load during this token's selection
     int t = blockIdx.x * nw + warp;
@@ -187,18 +224,16 @@ __global__ void __launch_bounds__(CNT, EPL <= 8 ? 2 : 1) route_kernel(const Args
             for (int i = 0; i < EPL; i++) f[i] = by_logit ? l[i] : (z == 0.f ? 0.f : expf(l[i] - m) / z);
         }
 #pragma unroll
-        for (int i = 0; i < EPL; i++) key[i] = e0 + i < E ? okey(f[i] + b[i]) : 0u;
-        uint32_t k1, k2;  // the lane's two best keys: most tokens take at most two experts from a lane
-        int i1, i2;
-        local2<EPL>(key, 0u, k1, i1, k2, i2);
+        for (int i = 0; i < EPL; i++) key[i] = okey(f[i] + b[i]);
+        Best b3 = local3<EPL>(key, ~0u, -1);
         if (GROUPS != ONE) {
             uint32_t g1 = 0, g2 = 0;  // two largest keys of the group that this lane ranks
             int mine;
             if (GROUPS == LANES) {
-                g1 = k1, g2 = k2;
+                g1 = b3.k1, g2 = b3.k2;
                 for (int o = 1; o < lanes_per; o <<= 1)
                     merge2(g1, g2, __shfl_xor_sync(0xffffffffu, g1, o), __shfl_xor_sync(0xffffffffu, g2, o));
-                mine = lane / lanes_per;
+                mine = lane >> lp_log;
             } else {
 #pragma unroll
                 for (int i = 0; i < EPL; i++)
@@ -212,12 +247,13 @@ __global__ void __launch_bounds__(CNT, EPL <= 8 ? 2 : 1) route_kernel(const Args
             const uint32_t gs = p.top2 && per > 1 ? okey(unkey(g1) + unkey(g2)) : g1;
             int rank = 0;
             if (GROUPS == LANES) {  // the group's lanes share the comparisons
-                for (int g = lane & (lanes_per - 1); g < p.groups + (lane & (lanes_per - 1)); g += lanes_per) {
-                    const uint32_t o = __shfl_sync(0xffffffffu, gs, g * lanes_per);
+                for (int g0 = 0; g0 < p.groups; g0 += lanes_per) {
+                    const int g = g0 + (lane & (lanes_per - 1));
+                    const uint32_t o = __shfl_sync(0xffffffffu, gs, g << lp_log);
                     if (g < p.groups) rank += (o > gs || (o == gs && g < mine)) ? 1 : 0;
                 }
                 for (int o = 1; o < lanes_per; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-                if (rank >= p.keep || mine >= p.groups) k1 = k2 = 0u;
+                if (rank >= p.keep || mine >= p.groups) b3.k1 = b3.k2 = b3.k3 = 0u;
             } else {
                 for (int g = 0; g < p.groups; g++) {
                     const uint32_t o = __shfl_sync(0xffffffffu, gs, g);
@@ -227,27 +263,17 @@ __global__ void __launch_bounds__(CNT, EPL <= 8 ? 2 : 1) route_kernel(const Args
 #pragma unroll
                 for (int i = 0; i < EPL; i++)
                     if (e0 + i < E && !((stay >> ((e0 + i) / per)) & 1u)) key[i] = 0u;
-                local2<EPL>(key, 0u, k1, i1, k2, i2);
+                b3 = local3<EPL>(key, ~0u, -1);
             }
         }
-        // top-k: the j-th choice goes to sel[j]
-        uint32_t gone = 0;
-        for (int j = 0; j < p.k; j++) {
-            const uint32_t top = __reduce_max_sync(0xffffffffu, k1);
-            const bool win = lane == __ffs(__ballot_sync(0xffffffffu, k1 == top)) - 1;
-            if (win) sel[j] = e0 + i1;
-            gone |= win ? 1u << i1 : 0u;
-            const bool again = EPL > 2 && win && k2 == 0u;
-            k1 = win ? k2 : k1, i1 = win ? i2 : i1, k2 = win ? 0u : k2;
-            if (again) local2<EPL>(key, gone, k1, i1, k2, i2);
-        }
-        __syncwarp();
-        const int choice = sel[lane];
-        __syncwarp();
+        const int choice = top_k<EPL>(key, b3, p.k, e0, lane);
         const bool on = lane < p.k;
         float s = 0.f;
         if (SIG) {
-            if (on) s = sigmoidf(to_f32(row[choice]));
+            const float l1[1] = {on ? to_f32(row[choice]) : 0.f};
+            float s1[1];
+            sigmoid_row<1>(l1, s1);
+            s = on ? s1[0] : 0.f;
         } else {
             const float lj = on ? to_f32(row[choice]) : -INFINITY;
             if (p.renorm) {  // the row's sum cancels: exponentials relative to the largest selected logit
@@ -379,7 +405,7 @@ static int launch_fwd(const Args& p, int grid, cudaStream_t st) {
     const int per = p.E / p.groups, lp = per / EPL;
     const int mode = p.groups == 1 ? ONE : per % EPL == 0 && (lp & (lp - 1)) == 0 ? LANES : ANY;
     const int nw = p.cluster ? CNT / 32 : NW;
-    const size_t smem = sizeof(uint32_t) * (nw * MAXK + (p.counts ? p.E : 0) + (mode == ANY ? nw * p.E : 0));
+    const size_t smem = sizeof(uint32_t) * ((p.counts ? p.E : 0) + (mode == ANY ? nw * p.E : 0));
     auto kern = p.sigmoid ? (mode == ONE     ? route_kernel<T, EPL, true, ONE>
                              : mode == LANES ? route_kernel<T, EPL, true, LANES>
                                              : route_kernel<T, EPL, true, ANY>)
