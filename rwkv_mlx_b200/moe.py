@@ -473,3 +473,17 @@ class Fp8MoE_CMix(nn.Module):
         """One token per sequence: x, x_prev (Bs, C) -> (Bs, C), as MoE_CMix.forward_rnn."""
         check_forward_only("Fp8MoE_CMix", x, self.parameters())
         return self._experts(x.contiguous(), x_prev, 1)[0]
+
+    def orthogonal_loss(self) -> torch.Tensor:
+        """As MoE_CMix: none for full experts (moe.py:241-242)."""
+        return torch.zeros((), device=self.x_k.device, dtype=torch.float32)
+
+
+def quantize_experts(model: nn.Module) -> nn.Module:
+    """Swap every :class:`MoE_CMix` of a model (in place) for its :class:`Fp8MoE_CMix`: prefill, RNN steps
+    and the captured graphs of the model then run their experts in 8 bits."""
+    for parent in list(model.modules()):
+        for name, child in list(parent.named_children()):
+            if isinstance(child, MoE_CMix):
+                setattr(parent, name, Fp8MoE_CMix(child))
+    return model

@@ -540,3 +540,41 @@ def test_moe_layer_in_8_bits(own_router, dtype):
         assert rel_rms(y.double().cpu().numpy().reshape(150, 256), ref.numpy()) < 0.05
     half = f8.half()                          # a module cast leaves the experts' bytes alone
     assert torch.equal(half.expert_weights()[0].view(torch.uint8), kq.view(torch.uint8))
+
+
+def test_model_with_experts_in_8_bits():
+    """quantize_experts swaps a model's full experts: prefill and decode agree with each other and, up to the
+    activations' quantisation (as in test_moe_layer_in_8_bits; it reaches the logits through the residual
+    stream, which it does not enlarge), with the 16-bit model on the same expert values; a captured decode step equals
+    the eager one."""
+    from rwkv_mlx_b200.model import RWKV, DecodeGraph, RWKVConfig, cast_for_inference, init_weights
+    from rwkv_mlx_b200.moe import Fp8MoE_CMix, MoE_CMix, quantize_experts
+
+    torch.manual_seed(0)
+    cfg = RWKVConfig(n_layer=2, n_embd=128, vocab_size=512, dim_ffn=256, moe_num_experts=4, moe_top_k=2, moe_mode="full")
+    m = init_weights(RWKV(cfg).cuda(), seed=1)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.add_(torch.randn(p.shape, generator=gen(2), device="cuda") * (0.05 if p.dim() > 1 else 0.02))
+        m.emb.weight.mul_(1000.0)
+    m = cast_for_inference(m)
+    idx = torch.randint(0, cfg.vocab_size, (3, 20), device="cuda", generator=gen(3))
+    with torch.no_grad():
+        for blk in m.blocks:  # values that e4m3 holds, so both models have the same experts
+            f8 = Fp8MoE_CMix(blk.ffn)
+            kq, ks, vq, vs = f8.expert_weights()
+            blk.ffn.expert_key.data = weight64(kq, ks).half().cuda()
+            blk.ffn.expert_val.data = weight64(vq, vs).half().cuda()
+        ref, aux = m(idx)
+        assert quantize_experts(m) is m and not any(isinstance(x, MoE_CMix) for x in m.modules())
+        y, aux8 = m(idx)
+        assert rel_rms(y.double().cpu().numpy(), ref.double().cpu().numpy()) < 0.05
+        assert abs(float(aux8) - float(aux)) < 0.05 * abs(float(aux)) + 1e-4
+        _, _, states = m.forward_with_state(idx[:, :16])
+        dec = torch.stack([m.forward_rnn_batch(idx[:, t], states) for t in range(16, 20)], 1)
+        assert rel_rms(dec.double().cpu().numpy(), y[:, 16:].double().cpu().numpy()) < 0.02
+        _, _, states = m.forward_with_state(idx[:, :16])
+        graph = DecodeGraph(m, [{k: v.clone() for k, v in st.items()} for st in states], idx[:, 16])
+        graph.step()
+        eager = m.forward_rnn_batch(idx[:, 16], states)
+        assert rel_rms(graph.logits.double().cpu().numpy(), eager.double().cpu().numpy()) < 1e-3
