@@ -3,7 +3,7 @@
 //   out[m, n] = epi( sum_kb as[kb, m] ws[g, n / 128, kb] sum_{k in block kb} a[m, k] w[g, n, k] )
 //
 // over the rows m in [offs[g], offs[g + 1]) of group g.  With few rows the product is bound
-// by reading the weights once, so this kernel streams them: a CTA owns 16 rows of W, its 8
+// by reading the weights once, so this kernel streams them: a CTA owns 16 or 32 rows of W, its
 // warps take the 128-blocks of K in turn, and every lane reads 16 consecutive bytes of a
 // weight row at a time straight into the operand registers of mma.sync m16n8k32 (weights as
 // the 16-row operand, tokens as the 8-column one).  The order of K inside a 64-byte piece
@@ -210,6 +210,7 @@ static int stream_launch(const GemmArgs& p, cudaStream_t st) {
     if (p.K >= 2048 && tiles <= 296) return stream_launch_t<TO, TX, 16, 1, 1, RELU2>(p, st);
     return stream_launch_t<TO, TX, 8, 1, 1, RELU2>(p, st);
 }
+
 int gemm_stream(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st) {
     if (epi == RELU2_Q) return RWKV_ERR_ARG;
     if (p.x) {  // one group, plain product
@@ -230,9 +231,10 @@ static int g_gemm_impl = 0;
 
 // Few rows: the weights are read once for every 32 rows of a group at most, and 16-row tiles of
 // W keep the SMs busy where 128 x 128 output tiles would not.  Measured, us, this kernel / tcgen05:
-// N = 4096, K = 1024, M = 16 4.7 / 6.2, 32 5.5 / 6.5, 64 9.3 / 6.6; 64 groups of N = 2048, K = 1024,
-// one row a group 19.3 / 19.4, four 35 / 32.
-static bool prefers_stream(int M, int G) { return M <= 32 || (G > 1 && M <= 2LL * G); }
+// N = 4096, K = 1024, M = 16 4.0 / 6.3, 32 4.3 / 6.4, 64 6.7 / 6.6; N = K = 4096, M = 32 9.0 / 13.5, 48 15.7 /
+// 13.7; 64 groups of N = 2048, K = 1024, one row a group 12.3 / 19.8, four 28 / 32, six 30 / 33 (and an
+// expert layer's hidden rows pass through memory in fp32 on this side).
+static bool prefers_stream(int M, int G) { return M <= 32 || (G > 1 && M <= 4LL * G); }
 
 }  // namespace fp8
 }  // namespace rwkv
@@ -259,7 +261,8 @@ bool known(int dtype) { return dtype == RWKV_F32 || dtype == RWKV_F16 || dtype =
 
 int gemm(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st) {
     const bool few = epi != fp8::RELU2_Q && (fp8::g_gemm_impl ? fp8::g_gemm_impl == 1 : fp8::prefers_stream(p.M, p.G));
-    return few ? fp8::gemm_stream(p, epi, out_dtype, st) : fp8::gemm_tc(p, epi, out_dtype, fp8::g_gemm_impl == 1 ? 0 : fp8::g_gemm_impl, st);
+    return few ? fp8::gemm_stream(p, epi, out_dtype, st)
+               : fp8::gemm_tc(p, epi, out_dtype, fp8::g_gemm_impl == 1 ? 0 : fp8::g_gemm_impl, st);
 }
 
 // Whether the streaming kernel takes a linear layer's x as it is and quantises it itself.  Not done

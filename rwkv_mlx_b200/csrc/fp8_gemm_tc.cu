@@ -27,7 +27,6 @@
 #include "fp8_gemm_pair.cuh"
 
 namespace rwkv {
-
 namespace fp8 {
 
 constexpr int BN = 128, NACC = 4, NS = 6, CTRL = 4096;
@@ -51,6 +50,7 @@ __device__ __forceinline__ void umma8(uint32_t d, uint64_t a, uint64_t b, uint32
         "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0), "r"(0), "r"(0), "r"(0)
         : "memory");
 }
+
 // A warp's 32 rows x HC columns to memory.  A lane holds one row, so stores straight from
 // registers would write 16 bytes of 32 rows at a time (measured: 16,000 cycles for a 128 x 256
 // tile of 16-bit outputs, four times its products at K = 1024).  The warp turns 64-byte pieces

@@ -22,7 +22,6 @@ constexpr int BM = 128, NDRAIN = 256, NTH = NDRAIN + 128, MAXG = 256;
 constexpr int REG_LAUNCH = 168, REG_DRAIN = 216, REG_ISSUE = 72;
 static_assert(REG_DRAIN * NDRAIN + REG_ISSUE * (NTH - NDRAIN) <= REG_LAUNCH * NTH, "register split");
 
-
 __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int Nn) {  // fp32 accumulate, both e4m3, K-major
     return (1u << 4) | ((uint32_t)(Nn >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }

@@ -84,9 +84,9 @@ __device__ __forceinline__ float wsum(float v) {
     return v;
 }
 
-// The lane's EPL logits of a row (experts past E: -inf).
+// The lane's EPL logits of a row (positions past E: `pad`).
 template <typename T, int EPL>
-__device__ __forceinline__ void load_row(const T* row, int e0, int E, bool vec, float (&l)[EPL]) {
+__device__ __forceinline__ void load_row(const T* row, int e0, int E, bool vec, float pad, float (&l)[EPL]) {
     constexpr int BYTES = EPL * sizeof(T), V = BYTES >= 16 ? 16 : BYTES, PER = V / sizeof(T);
     if (vec && e0 + EPL <= E) {
 #pragma unroll
@@ -101,7 +101,7 @@ __device__ __forceinline__ void load_row(const T* row, int e0, int E, bool vec, 
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < EPL; i++) l[i] = e0 + i < E ? to_f32(row[e0 + i]) : -INFINITY;
+        for (int i = 0; i < EPL; i++) l[i] = e0 + i < E ? to_f32(row[e0 + i]) : pad;
     }
 }
 
@@ -195,15 +195,16 @@ __global__ void __launch_bounds__(CNT, EPL <= 8 ? 2 : 1) route_kernel(const Args
     // positions past E get -inf, so their keys rank below or tie with every expert's, which have the lower index
     for (int i = 0; i < EPL; i++) b[i] = e0 + i >= E ? -INFINITY : p.bias ? p.bias[e0 + i] : 0.f;
 
+    constexpr float PAD = SIG ? 0.f : -INFINITY;  // outside a softmax's sum; no large d for sigmoid_row
     float next[EPL];  // the next token's logits load during this token's selection
     int t = blockIdx.x * nw + warp;
-    if (t < p.n) load_row<T, EPL>(reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld, e0, E, p.vec, next);
+    if (t < p.n) load_row<T, EPL>(reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld, e0, E, p.vec, PAD, next);
     for (; t < p.n; t += gridDim.x * nw) {
         const T* row = reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld;
         float l[EPL];
 #pragma unroll
         for (int i = 0; i < EPL; i++) l[i] = next[i];
-        if (t + (int)gridDim.x * nw < p.n) load_row<T, EPL>(row + (long long)gridDim.x * nw * p.ld, e0, E, p.vec, next);
+        if (t + (int)gridDim.x * nw < p.n) load_row<T, EPL>(row + (long long)gridDim.x * nw * p.ld, e0, E, p.vec, PAD, next);
         float m = 0.f, z = 0.f;  // softmax: row maximum (0 for a row of -inf) and sum
         if (!SIG && (!by_logit || !p.renorm)) {
             m = -INFINITY;
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(NT) route_bwd_kernel(const BwdArgs p) {
         __syncwarp();
         if (dense) {
             float l[EPL], m = -INFINITY, z = 0.f;
-            load_row<T, EPL>(row, e0, E, p.vec, l);
+            load_row<T, EPL>(row, e0, E, p.vec, -INFINITY, l);
 #pragma unroll
             for (int i = 0; i < EPL; i++) m = (l[i] > m || l[i] != l[i]) ? l[i] : m;
             m = wmax(m);
