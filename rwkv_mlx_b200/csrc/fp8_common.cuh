@@ -19,6 +19,24 @@ __device__ __forceinline__ float clamp_amax(float a) { return fmaxf(a, FP8_TINY)
 __device__ __forceinline__ float quant_mul(float a) { return __fmul_rn(__frcp_rn(a), E4M3_MAX); }
 __device__ __forceinline__ float dequant_scale(float a) { return __fmul_rn(a, 1.f / E4M3_MAX); }
 
+// Chained launches (a layer's quantisation and products): a kernel lets its successor start at once,
+// and the successor does what needs nothing of it (its barriers, its first weights) and then waits
+// until it has completed.  Only kernels launched with launch_chained() start early; for all others both
+// are no-ops.  What a chain's first kernel finds complete (weights, offsets) may be read before the wait.
+__device__ __forceinline__ void chain_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+inline int launch_chained(bool chained, void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid, cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cfg.attrs = &at, cfg.numAttrs = chained ? 1 : 0;
+    return set_cuda_error(cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...));
+}
+
 // Two floats to two e4m3 bytes (lower address: lo), round to nearest even.
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint16_t r;

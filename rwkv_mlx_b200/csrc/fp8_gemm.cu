@@ -57,6 +57,9 @@ __global__ void __launch_bounds__(NW * 32) gemm_stream_kernel(const GemmArgs p) 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
     const int g = blockIdx.y, n0 = blockIdx.x * ROWS;
     const int r0 = p.offs ? max(p.offs[g], 0) : 0, r1 = p.offs ? min(p.offs[g + 1], p.M) : p.M;
+    // (first loads of the weights before this wait cost the kernel 30 registers and more time than they won)
+    chain_let_next();
+    chain_wait();
     if (r0 >= r1) return;
     const int nkb = (p.K + BLK - 1) / BLK;
     const int pitch = nkb * BLK + 16;  // eight rows' pieces of one column lie in different banks
@@ -107,6 +110,23 @@ __global__ void __launch_bounds__(NW * 32) gemm_stream_kernel(const GemmArgs p) 
             for (int j = 0; j < NT8; j++)
 #pragma unroll
                 for (int c = 0; c < 4; c++) acc[r][j][c] = 0.f;
+        auto products = [&]() {
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int j = 0; j < NT8; j++) {
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint4 x = wv[r][0][h], y = wv[r][1][h], b = av[j][h];
+                        mma_e4m3(part, x.x, y.x, x.y, y.y, b.x, b.y);
+                        mma_e4m3(part, x.z, y.z, x.w, y.w, b.z, b.w);
+                    }
+                    const float s0 = s[j][0] * sb, s1 = s[j][1] * sb;
+                    acc[r][j][0] += part[0] * s0, acc[r][j][1] += part[1] * s1;
+                    acc[r][j][2] += part[2] * s0, acc[r][j][3] += part[3] * s1;
+                }
+        };
         if constexpr (SELF) {
             if (warp < nkb) load_w(warp);
             const int ntok = min(8, r1 - m0), l = lane & 15;
@@ -143,21 +163,7 @@ __global__ void __launch_bounds__(NW * 32) gemm_stream_kernel(const GemmArgs p) 
         for (int kb = warp; kb < nkb; kb += NW) {
             if (!SELF || kb != warp) load_w(kb);
             load_a(kb);
-#pragma unroll
-            for (int r = 0; r < RT; r++)
-#pragma unroll
-                for (int j = 0; j < NT8; j++) {
-                    float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint4 x = wv[r][0][h], y = wv[r][1][h], b = av[j][h];
-                        mma_e4m3(part, x.x, y.x, x.y, y.y, b.x, b.y);
-                        mma_e4m3(part, x.z, y.z, x.w, y.w, b.z, b.w);
-                    }
-                    const float s0 = s[j][0] * sb, s1 = s[j][1] * sb;
-                    acc[r][j][0] += part[0] * s0, acc[r][j][1] += part[1] * s1;
-                    acc[r][j][2] += part[2] * s0, acc[r][j][3] += part[3] * s1;
-                }
+            products();
         }
 #pragma unroll
         for (int r = 0; r < RT; r++)
@@ -192,13 +198,12 @@ static int stream_launch_t(const GemmArgs& p, cudaStream_t st) {
             const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
             if (err != cudaSuccess) return set_cuda_error(err);
         }
-        kern<<<grid, NW * 32, smem, st>>>(p);
+        return launch_chained(p.chained, kern, grid, NW * 32, smem, st, p);
     } else {
         auto kern = p.K % 16 == 0 ? gemm_stream_kernel<TO, TX, NW, RT, NT8, true, RELU2>
                                   : gemm_stream_kernel<TO, TX, NW, RT, NT8, false, RELU2>;
-        kern<<<grid, NW * 32, 0, st>>>(p);
+        return launch_chained(p.chained, kern, grid, NW * 32, 0, st, p);
     }
-    return check_launch();
 }
 // Measured with the weights out of L2 (e4m3 rows): 4096 x 1024 2.3 us with 8 warps; 4096 x 4096 7.5 us with 8,
 // 6.3 with 16; 8192 x 8192 17 with 8, 18 with 16; 64 groups of 2048 x 1024 with 36 in use 19.7 us with 8 warps, 15.5
@@ -207,7 +212,7 @@ template <typename TO, typename TX, bool RELU2>
 static int stream_launch(const GemmArgs& p, cudaStream_t st) {
     const long long tiles = (long long)p.G * ((p.N + SROWS - 1) / SROWS);
     if (tiles >= 2048) return stream_launch_t<TO, TX, 4, 2, 1, RELU2>(p, st);
-    if (p.K >= 2048 && tiles <= 296) return stream_launch_t<TO, TX, 16, 1, 1, RELU2>(p, st);
+    if (p.K >= 2048 && tiles <= 2 * sm_count()) return stream_launch_t<TO, TX, 16, 1, 1, RELU2>(p, st);
     return stream_launch_t<TO, TX, 8, 1, 1, RELU2>(p, st);
 }
 
@@ -316,8 +321,9 @@ extern "C" int rwkv_fp8_linear(const void* x, long long ldx, const void* w, long
     float* qs = (float*)(q + rows_bytes(M, K));
     rc = rwkv_quantize_fp8_rows(x, ldx, q, pitch16(K), qs, M, K, dtype, stream);
     if (rc) return rc;
-    return gemm({q, pitch16(K), qs, (const uint8_t*)w, ldw, 0, w_scale, nullptr, out, ldo, nullptr, M, N, K, 1},
-                fp8::STORE, dtype, (cudaStream_t)stream);
+    GemmArgs p{q, pitch16(K), qs, (const uint8_t*)w, ldw, 0, w_scale, nullptr, out, ldo, nullptr, M, N, K, 1};
+    p.chained = true;
+    return gemm(p, fp8::STORE, dtype, (cudaStream_t)stream);
 }
 
 extern "C" size_t rwkv_fp8_experts_workspace_size(int M, int C, int D, int E) {
@@ -351,16 +357,18 @@ extern "C" int rwkv_fp8_experts(const void* x, long long ldx, const void* key, l
     rc = rwkv_quantize_fp8_rows(x, ldx, q, pitch16(C), qs, M, C, dtype, stream);
     if (rc) return rc;
     GemmArgs p{q, pitch16(C), qs, (const uint8_t*)key, ldk, key_gs, key_scale, offs, hq, pitch16(D), hs, M, D, C, E};
+    p.chained = true;
     if (few) {  // 16 columns a CTA: a block's maximum is not in one place, so the hidden rows pass through fp32
         p.out = at, p.ldo = D, p.os = nullptr;
         rc = gemm(p, fp8::RELU2, RWKV_F32, st);
-        if (!rc) rc = rwkv_quantize_fp8_rows(at, D, hq, pitch16(D), hs, M, D, RWKV_F32, stream);
+        if (!rc) rc = fp8::quantize_rows(at, nullptr, D, hq, pitch16(D), hs, M, D, RWKV_F32, true, st);
     } else {
         rc = gemm(p, fp8::RELU2_Q, dtype, st);
     }
     if (rc) return rc;
-    return gemm({hq, pitch16(D), hs, (const uint8_t*)val, ldv, val_gs, val_scale, offs, out, ldo, nullptr, M, C, D, E},
-                fp8::STORE, dtype, st);
+    GemmArgs v{hq, pitch16(D), hs, (const uint8_t*)val, ldv, val_gs, val_scale, offs, out, ldo, nullptr, M, C, D, E};
+    v.chained = true;
+    return gemm(v, fp8::STORE, dtype, st);
 }
 
 extern "C" int rwkv_fp8_set_gemm_impl(int impl) {

@@ -21,11 +21,22 @@ struct GemmArgs {
     int M, N, K, G;
     const void* x = nullptr;  // gemm_stream: rows of the output's type, still to be quantised, instead of a and as
     long long ldx = 0;
+    bool chained = false;  // the launch before this one is part of the same chain
 };
+
+// rwkv_quantize_fp8_rows as a member of a chain.
+int quantize_rows(const void* x, const void* u, long long ldx, void* q, long long ldq, float* scale, int M, int K,
+                  int dtype, bool chained, cudaStream_t st);
 
 // gemm_stream quantises x itself (in every CTA) for at most this many rows and K up to SELF_K, a
 // multiple of 16.
 constexpr int SELF_ROWS = 8, SELF_K = 8192;
+
+inline int sm_count() {
+    int dev = 0, n = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n;
+}
 
 int gemm_stream(const GemmArgs& p, int epi, int out_dtype, cudaStream_t st);
 int gemm_tc(const GemmArgs& p, int epi, int out_dtype, int impl, cudaStream_t st);

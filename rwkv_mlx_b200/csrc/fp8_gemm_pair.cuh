@@ -103,6 +103,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp8::NTH, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     load_offsets(cs.groups, p, tid);
+    chain_let_next();
+    chain_wait();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -351,8 +353,7 @@ static int launch_pair(const GemmArgs& p, int pairs, cudaStream_t st) {
     auto kern = fp8_gemm_pair_kernel<EPI, TO>;
     const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM);
     if (err != cudaSuccess) return set_cuda_error(err);
-    kern<<<2 * pairs, NTH, PAIR_SMEM, st>>>(ma, mw, mo, p, tma_out);
-    return check_launch();
+    return launch_chained(p.chained, kern, 2 * pairs, NTH, PAIR_SMEM, st, ma, mw, mo, p, tma_out);
 }
 
 static int gemm_pair(const GemmArgs& p, int epi, int out_dtype, int pairs, cudaStream_t st) {

@@ -127,6 +127,8 @@ __global__ void __launch_bounds__(fp8::NTH, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     load_offsets(cs.groups, p, tid);
+    chain_let_next();
+    chain_wait();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -310,8 +312,7 @@ static int launch_tc(const GemmArgs& p, int grid, cudaStream_t st) {
     const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (err != cudaSuccess) return set_cuda_error(err);
     const int vec = aligned(p.out, 16) && (p.ldo * (int)sizeof(TO)) % 16 == 0;
-    kern<<<grid, NTH, SMEM, st>>>(ma, mw, p, vec);
-    return check_launch();
+    return launch_chained(p.chained, kern, grid, NTH, SMEM, st, ma, mw, p, vec);
 }
 
 // impl: 0 automatic, 2 one CTA a tile, 3 CTA pairs.  Measured, us, one CTA / pair: 1024 x 1024 x 1024

@@ -7,7 +7,7 @@
 // the scales go out as (blocks of K, rows), rows contiguous, which is the order in
 // which the product's epilogue (one thread per row) reads them.  Measured: 32768 x 1024 bf16
 // 18.6 us = 5.5 TB/s, 16384 x 4096 34.6 us = 5.9 TB/s (0.85 and 0.91 of the copy rate).
-#include "fp8_common.cuh"
+#include "fp8_gemm.cuh"
 
 namespace rwkv {
 namespace fp8 {
@@ -30,6 +30,8 @@ __global__ void __launch_bounds__(QT)
     const T *xr = x + (long long)row * ldx, *ur = GRAD ? u + (long long)row * ldx : nullptr;
     uint8_t* qr = q + (long long)row * ldq;
     __shared__ float sm[QU][QROWS];
+    chain_let_next();
+    chain_wait();
     uint4 raw[QU][NV], rawu[GRAD ? QU : 1][NV];
 #pragma unroll
     for (int b = 0; b < QU; b++) {
@@ -160,13 +162,8 @@ __global__ void __launch_bounds__(256)
     if (threadIdx.x == 0) scale[((long long)g * gridDim.y + nb) * gridDim.x + kb] = dequant_scale(a);
 }
 
-}  // namespace fp8
-}  // namespace rwkv
-
-using namespace rwkv;
-
-static int quantize_rows(const void* x, const void* u, long long ldx, void* q, long long ldq, float* scale, int M, int K,
-                         int dtype, void* stream) {
+int quantize_rows(const void* x, const void* u, long long ldx, void* q, long long ldq, float* scale, int M, int K,
+                  int dtype, bool chained, cudaStream_t st) {
     if (dtype != RWKV_F32 && dtype != RWKV_F16 && dtype != RWKV_BF16) return RWKV_ERR_DTYPE;
     if (M < 0 || K <= 0 || ldx < K || ldq < K) return RWKV_ERR_SHAPE;
     if (M == 0) return RWKV_OK;
@@ -174,26 +171,31 @@ static int quantize_rows(const void* x, const void* u, long long ldx, void* q, l
     if (!aligned(q, 8) || ldq % 8) return RWKV_ERR_ALIGN;
     const int es = dtype == RWKV_F32 ? 4 : 2;
     const bool vec = aligned(x, 16) && aligned(u, 16) && (ldx * es) % 16 == 0 && K % 8 == 0;
-    const int nkb = (K + fp8::BLK - 1) / fp8::BLK;
-    const dim3 grid((M + fp8::QROWS - 1) / fp8::QROWS, (nkb + fp8::QU - 1) / fp8::QU);
+    const int nkb = (K + BLK - 1) / BLK;
+    const dim3 grid((M + QROWS - 1) / QROWS, (nkb + QU - 1) / QU);
     if (grid.y > 65535) return RWKV_ERR_SHAPE;
     RWKV_DISPATCH_DTYPE(dtype, T, {
-        auto kern = u ? (vec ? fp8::quant_rows_kernel<T, true, true> : fp8::quant_rows_kernel<T, false, true>)
-                      : (vec ? fp8::quant_rows_kernel<T, true, false> : fp8::quant_rows_kernel<T, false, false>);
-        kern<<<grid, fp8::QT, 0, (cudaStream_t)stream>>>((const T*)x, (const T*)u, ldx, (uint8_t*)q, ldq, scale, M, K);
+        auto kern = u ? (vec ? quant_rows_kernel<T, true, true> : quant_rows_kernel<T, false, true>)
+                      : (vec ? quant_rows_kernel<T, true, false> : quant_rows_kernel<T, false, false>);
+        return launch_chained(chained, kern, grid, QT, 0, st, (const T*)x, (const T*)u, ldx, (uint8_t*)q, ldq, scale, M, K);
     });
-    return check_launch();
+    return RWKV_ERR_DTYPE;
 }
+
+}  // namespace fp8
+}  // namespace rwkv
+
+using namespace rwkv;
 
 extern "C" int rwkv_quantize_fp8_rows(const void* x, long long ldx, void* q, long long ldq, float* scale, int M, int K,
                                       int dtype, void* stream) {
-    return quantize_rows(x, nullptr, ldx, q, ldq, scale, M, K, dtype, stream);
+    return fp8::quantize_rows(x, nullptr, ldx, q, ldq, scale, M, K, dtype, false, (cudaStream_t)stream);
 }
 
 extern "C" int rwkv_quantize_fp8_relu_sq_grad(const void* dh, const void* u, long long ld, void* q, long long ldq,
                                               float* scale, int M, int K, int dtype, void* stream) {
     if (M > 0 && !u) return RWKV_ERR_ARG;
-    return quantize_rows(dh, u, ld, q, ldq, scale, M, K, dtype, stream);
+    return fp8::quantize_rows(dh, u, ld, q, ldq, scale, M, K, dtype, false, (cudaStream_t)stream);
 }
 
 extern "C" int rwkv_quantize_fp8_weight(const void* w, void* q, long long ldq, float* scale, int G, int N, int K,

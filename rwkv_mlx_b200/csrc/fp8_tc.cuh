@@ -139,11 +139,6 @@ inline long long row_tiles(int M, int G, int rows) {
     const long long most = (M + rows - 1) / rows + (G > 1 ? G - 1 : 0);
     return most < M ? most : M;
 }
-inline int sm_count() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n;
-}
 
 }  // namespace fp8
 }  // namespace rwkv

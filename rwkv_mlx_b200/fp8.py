@@ -149,8 +149,8 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
     e4m3 operands and their scales stand for; fp32 accumulation, one rounding to ``out_dtype``.
 
     a (M, K) with a_scale as :func:`quantize_fp8_rows` returns them, w (N, K) or (G, N, K) with w_scale
-    as :func:`quantize_fp8_weight` does.  ``offsets`` (G + 1,) int32 on the device, ascending, or None for
-    one group over all rows; rows outside every group are left as they were in ``out``.  ``relu_sq``:
+    as :func:`quantize_fp8_weight` does.  ``offsets`` (G + 1,) int32 on the device, ascending (G <= 256), or None
+    for one group over all rows; rows outside every group are left as they were in ``out``.  ``relu_sq``:
     relu(.)^2 of the fp32 product.  No gradient (see :func:`fp8_linear`)."""
     if out is None:
         out = torch.empty((a.shape[0], w.shape[-2]), device=a.device, dtype=out_dtype)
