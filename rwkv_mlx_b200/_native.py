@@ -12,6 +12,7 @@ import os
 from pathlib import Path
 
 import torch
+from torch.autograd.function import once_differentiable
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "librwkv_b200.so"
 
@@ -179,6 +180,17 @@ def stream_ptr(device=None):
     if device is not None and device.index is not None:
         return torch._C._cuda_getCurrentRawStream(device.index)  # the same handle, without a Stream object
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def first_order(backward):
+    """``once_differentiable`` whose wrapping is paid for only where a graph of the backward pass is asked
+    for (there the result raises when it is differentiated again)."""
+    guarded = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
 
 
 def on_device(dev: torch.device):

@@ -14,7 +14,6 @@ the rows contiguous, weight scales (..., ceil(N / 128), ceil(K / 128)) fp32 cont
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -198,7 +197,7 @@ class _Linear(torch.autograd.Function):
         return _linear(x2d, w, w_scale)
 
     @staticmethod
-    @once_differentiable
+    @nat.first_order
     def backward(ctx, dy):
         return _linear(nat.rows_2d(dy), *ctx.saved_tensors), None, None, None, None
 
@@ -246,7 +245,7 @@ class _Experts(torch.autograd.Function):
         return _experts(x, *weights, offsets, *dims)
 
     @staticmethod
-    @once_differentiable
+    @nat.first_order
     def backward(ctx, dy):
         x, offsets, key, key_scale, key_t, key_t_scale, value_t, value_t_scale = ctx.saved_tensors
         # u again rather than kept from the forward pass (there it never leaves the key product's kernel)

@@ -11,7 +11,6 @@ reference.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -46,7 +45,7 @@ class _Route(torch.autograd.Function):
         return inds, weights, counts
 
     @staticmethod
-    @once_differentiable
+    @nat.first_order
     def backward(ctx, _dinds, dweights, _dcounts=None):
         if dweights is None:
             return (None,) * 10
