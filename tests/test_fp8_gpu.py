@@ -256,6 +256,27 @@ def test_linear_and_its_gradient(dtype, M):
         assert torch.equal(fp8_linear(x, wq, ws), y)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("K", [16, 144, 1040, 4096, 8192, 8208])
+@pytest.mark.parametrize("M", [1, 3, 8, 9])
+def test_linear_of_few_rows(dtype, K, M):
+    """Rows that the product's own kernel quantises (up to 8, K a multiple of 16 up to 8192) against the two calls in a row:
+    the same bytes and the same sums, so the same result; odd pitches and bases included."""
+    from rwkv_mlx_b200.fp8 import fp8_linear, fp8_matmul, quantize_fp8_rows, quantize_fp8_weight
+
+    for N in (40, 300):
+        wq, ws = quantize_fp8_weight(torch.randn(N, K, device="cuda", generator=gen(N)))
+        wide = data(M, K + 7, M, dtype)
+        for x in (wide[:, :K].contiguous(), wide[:, 3:3 + K], wide[:, 1:1 + K]):
+            y = fp8_linear(x, wq, ws)
+            assert torch.equal(y, fp8_matmul(*quantize_fp8_rows(x), wq, ws, out_dtype=dtype))
+    x = torch.randn(M, K, device="cuda", generator=gen(1)).to(dtype)
+    x[0] = 0
+    x[-1, K // 2] = math.nan
+    y = fp8_linear(x, wq, ws)
+    assert torch.isnan(y[-1]).all() and (M == 1 or (y[0] == 0).all()) and torch.isfinite(y[:-1]).all()
+
+
 def test_linear_gradient_against_differences():
     """dy and the steps lie on values that e4m3 holds exactly in every block, so quantisation is the identity and the
     product is linear: differences of float64-exact values."""
