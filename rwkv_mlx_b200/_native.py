@@ -1,4 +1,5 @@
-"""ctypes binding of the C-ABI library ``_lib/librwkv_b200.so`` (include/rwkv_b200.h).
+"""ctypes binding of the C-ABI library ``_lib/librwkv_b200.so`` (include/rwkv_b200.h), and the loader
+of ``_lib/_rwkv_host.so``, which calls some of its entry points from C++.
 
 The library is the only compute path: if it is missing, or no CUDA device is
 present, the public functions raise instead of falling back to anything else.
@@ -8,13 +9,14 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib.util
 import os
 from pathlib import Path
 
 import torch
-from torch.autograd.function import once_differentiable
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "librwkv_b200.so"
+HOST_PATH = LIB_PATH.with_name("_rwkv_host.so")
 
 STATUS = {
     0: "ok",
@@ -133,6 +135,25 @@ def load(path: Path | None = None) -> ctypes.CDLL:
     return _lib
 
 
+_host = None
+
+
+def host():
+    """The module ``_lib/_rwkv_host.so`` (csrc/host), bound to this library's entry points: the expert-layer
+    operators' host side in C++.  It is their only path and needs no GPU to load."""
+    global _host
+    if _host is None:
+        if not HOST_PATH.exists():
+            raise RwkvNativeError(f"{HOST_PATH} not found: build it with `python -m rwkv_mlx_b200.build` (there is no fallback)")
+        spec = importlib.util.spec_from_file_location("_rwkv_host", HOST_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        L = load()
+        mod.bind({n: ctypes.cast(getattr(L, n), _P).value for n in SIGNATURES}, RwkvNativeError, STATUS)
+        _host = mod
+    return _host
+
+
 _has_gpu = False
 
 
@@ -158,13 +179,19 @@ KERNELS_PER_CALL = {
     "rwkv_fp8_gemm": 1, "rwkv_fp8_linear": 1, "rwkv_fp8_experts": 3,  # at least: few or many rows take one more
     "rwkv_grouped_gemm": 1, "rwkv_head_ce_stats": 2, "rwkv_head_ce_grad": 1,
 }
-launch_count = 0
+_launches = 0
+
+
+def __getattr__(name):
+    if name == "launch_count":
+        return _launches + (_host.launches() if _host is not None else 0)
+    raise AttributeError(name)
 
 
 def check(rc: int, what: str, kernels: int | None = None) -> None:
-    global launch_count
+    global _launches
     if rc == 0:
-        launch_count += KERNELS_PER_CALL.get(what, 0) if kernels is None else kernels
+        _launches += KERNELS_PER_CALL.get(what, 0) if kernels is None else kernels
     if rc != 0:
         msg = STATUS.get(rc, f"status {rc}")
         if rc == 4:
@@ -180,17 +207,6 @@ def stream_ptr(device=None):
     if device is not None and device.index is not None:
         return torch._C._cuda_getCurrentRawStream(device.index)  # the same handle, without a Stream object
     return torch.cuda.current_stream(device).cuda_stream
-
-
-def first_order(backward):
-    """``once_differentiable`` whose wrapping is paid for only where a graph of the backward pass is asked
-    for (there the result raises when it is differentiated again)."""
-    guarded = once_differentiable(backward)
-
-    def call(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-
-    return call
 
 
 def on_device(dev: torch.device):

@@ -5,7 +5,8 @@ under ``csrc/`` is compiled for ``-gencode arch=compute_100a,code=sm_100a`` into
 an object under ``_build/`` and linked into one shared library with the CUDA
 runtime linked statically, so the library carries no dependency on the
 torch-bundled runtime.  Rebuilds only what changed (sources or headers newer
-than the object).
+than the object).  ``csrc/host/`` becomes ``_lib/_rwkv_host.so`` with the host compiler, a Python module
+that links against PyTorch and calls the library's entry points.
 """
 
 from __future__ import annotations
@@ -14,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -22,6 +24,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "_lib" / "librwkv_b200.so"
+HOST_LIB = PKG / "_lib" / "_rwkv_host.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -56,12 +59,46 @@ def _compile(src: Path, debug: bool) -> Path:
     return obj
 
 
+def gxx() -> str:
+    """The system's compiler ($RWKV_HOST_CXX: another), not $CXX: one that links libstdc++ statically gives a
+    module whose streams crash beside the shared libstdc++ that PyTorch uses."""
+    for cand in (os.environ.get("RWKV_HOST_CXX"), "/usr/bin/g++", shutil.which("g++")):
+        if cand and Path(cand).exists():
+            return cand
+    raise RuntimeError("g++ not found")
+
+
+def _build_host() -> None:
+    src = CSRC / "host" / "expert_ops.cpp"
+    newest = max(src.stat().st_mtime, (ROOT / "include" / "rwkv_b200.h").stat().st_mtime)
+    if HOST_LIB.exists() and HOST_LIB.stat().st_mtime >= newest:
+        return
+    import torch
+    from torch.utils import cpp_extension
+
+    inc = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], Path(nvcc()).resolve().parents[1] / "include",
+           ROOT / "include"]
+    tmp = HOST_LIB.with_suffix(".so.tmp")
+    cmd = [gxx(), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in inc), str(src),
+           "-o", str(tmp), *(f"-L{p}" for p in cpp_extension.library_paths()),
+           "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_python", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {src.name}:\n{res.stderr}")
+    if b"libstdc++.so" not in tmp.read_bytes():
+        raise RuntimeError(f"{cmd[0]} linked {src.name} without the shared libstdc++")
+    os.replace(tmp, HOST_LIB)
+
+
 def build(verbose: bool = False, debug: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     LIB.parent.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.cu"))
-    with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with ThreadPoolExecutor(max_workers=min(9, len(srcs) + 1)) as ex:
+        host = ex.submit(_build_host)
         objs = list(ex.map(lambda s: _compile(s, debug), srcs))
+        host.result()
     if not LIB.exists() or LIB.stat().st_mtime < max(o.stat().st_mtime for o in objs):
         tmp = LIB.with_suffix(".so.tmp")
         cmd = [nvcc()] + ARCH + ["-shared", "-cudart", "static", "-Xcompiler", "-fPIC",
@@ -71,7 +108,7 @@ def build(verbose: bool = False, debug: bool = False) -> Path:
             raise RuntimeError(f"link failed:\n{res.stderr}")
         os.replace(tmp, LIB)
     if verbose:
-        print(f"built {LIB}")
+        print(f"built {LIB}, {HOST_LIB}")
     return LIB
 
 

@@ -1,0 +1,418 @@
+// Host side of the expert-layer operators: argument checks, outputs, workspaces and autograd around the
+// C entry points of rwkv_b200.h, for calls whose GPU time is a few microseconds.  The same steps in Python
+// over ctypes bounded them.  Host time a call, before -> here, in us: routing 14 -> 7, row quantisation
+// 12 -> 6, a linear layer of 4 rows 13 -> 5 and of 64 rows 17 -> 9, the experts 27 -> 12; with the
+// gradient, routing 94 -> 52, the linear layer of 64 rows 108 -> 63 and the experts 211 -> 90, of which the
+// autograd engine is most (it runs a Python backward with the interpreter lock, taken on its own thread).
+//
+// The entry points come as addresses from the Python binding, which has loaded the library: this
+// module links against PyTorch only.  Bad arguments raise ValueError, a failing entry point
+// RwkvNativeError, as in the binding.
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <atomic>
+#include <limits>
+#include <map>
+#include <sstream>
+#include <stdexcept>
+#include <variant>
+
+#include "rwkv_b200.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// ------------------------------------------------------------------ binding
+
+#define ENTRY_POINTS(X)                                                                                  \
+    X(rwkv_route_experts) X(rwkv_route_experts_backward) X(rwkv_quantize_fp8_rows)                       \
+    X(rwkv_quantize_fp8_relu_sq_grad) X(rwkv_fp8_gemm) X(rwkv_fp8_linear) X(rwkv_fp8_linear_workspace_size) \
+    X(rwkv_fp8_experts) X(rwkv_fp8_experts_workspace_size) X(rwkv_last_error)
+#define DECLARE(name) decltype(&::name) p_##name = nullptr;
+ENTRY_POINTS(DECLARE)
+
+PyObject* g_native_error = nullptr;
+std::map<int, std::string> g_status;
+std::atomic<long long> g_launches{0};
+
+void bind(const py::dict& addresses, const py::object& native_error, const std::map<int, std::string>& status) {
+#define BIND(name) \
+    p_##name = reinterpret_cast<decltype(p_##name)>(addresses[#name].cast<uintptr_t>());
+    ENTRY_POINTS(BIND)
+    Py_XDECREF(g_native_error);
+    g_native_error = native_error.inc_ref().ptr();
+    g_status = status;
+}
+
+// ------------------------------------------------------------------ errors and small helpers
+
+template <typename... A>
+[[noreturn]] void bad(const A&... parts) {
+    std::ostringstream s;
+    (s << ... << parts);
+    throw py::value_error(s.str());
+}
+// (the operators and their backward passes run without the interpreter lock)
+[[noreturn]] void native_error(const std::string& msg) {
+    py::gil_scoped_acquire gil;
+    PyErr_SetString(g_native_error, msg.c_str());
+    python_error e;
+    e.persist();
+    throw e;
+}
+void check(int rc, const char* what, int kernels) {
+    if (rc == 0) {
+        g_launches += kernels;
+        return;
+    }
+    const auto it = g_status.find(rc);
+    std::string msg = std::string(what) + " failed: " + (it == g_status.end() ? "status " + std::to_string(rc) : it->second);
+    if (rc == RWKV_ERR_CUDA) msg += std::string(": ") + p_rwkv_last_error();
+    native_error(msg);
+}
+
+int dtype_code(const Tensor& t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return RWKV_F32;
+        case at::kHalf: return RWKV_F16;
+        case at::kBFloat16: return RWKV_BF16;
+        default: {
+            std::ostringstream s;
+            s << "unsupported dtype " << t.scalar_type();
+            native_error(s.str());
+        }
+    }
+}
+void on_gpu(const char* name, const Tensor& t) {
+    if (t.is_cuda()) return;
+    if (c10::cuda::device_count() == 0) native_error("rwkv_mlx_b200 kernels need a CUDA device (no CPU fallback)");
+    bad(name, ": the tensors must be on a CUDA device, not ", t.device());
+}
+void* stream(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+int64_t blocks(int64_t n) { return (n + 127) / 128; }
+int64_t pitch16(int64_t n) { return (n + 15) / 16 * 16; }
+// (.., C) as (rows, C) with unit column stride, copied only where no view has that.
+Tensor rows_2d(const Tensor& t) {
+    Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+    return r.stride(1) == 1 && r.stride(0) >= r.size(1) ? r : r.contiguous();
+}
+// Row pitch in elements (any multiple of 16 does for a single row).
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : pitch16(t.size(1)); }
+int as_int(const char* name, int64_t n) {
+    if (n > std::numeric_limits<int>::max()) bad(name, ": ", n, " is more than a size can be");
+    return (int)n;
+}
+Tensor matrix(int64_t rows, int64_t cols, const Tensor& like, at::ScalarType type, int64_t pitch = 0) {
+    return at::empty_strided({rows, cols}, {pitch ? pitch : cols, 1}, like.options().dtype(type));
+}
+Tensor empty_e4m3(int64_t rows, int64_t cols, const Tensor& like) {
+    return matrix(rows, cols, like, at::kFloat8_e4m3fn, pitch16(cols));
+}
+Tensor empty_scale(int64_t rows, int64_t cols, const Tensor& like) {  // rows contiguous
+    return at::empty_strided({rows, blocks(cols)}, {1, std::max<int64_t>(rows, 1)}, like.options().dtype(at::kFloat));
+}
+bool wants_grad(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+
+// What a backward pass returns for an input: where a graph of the pass itself is asked for, a value that
+// raises when it is differentiated again (the entry points have no second derivatives).
+Tensor once(const Tensor& grad) {
+    if (!at::GradMode::is_enabled()) return grad;
+    Tensor v = grad.detach();
+    v.set_requires_grad(true);
+    auto err = std::make_shared<torch::autograd::DelayedError>("this backward pass can be differentiated only once", 1);
+    return (*err)({v})[0];
+}
+
+// ------------------------------------------------------------------ routing
+
+struct RouteOpts {
+    int k, sigmoid, groups, keep, top2, renorm;
+    double scale;
+    bool counts;
+};
+
+std::tuple<Tensor, Tensor, Tensor> route_forward(const Tensor& l, const std::optional<Tensor>& bias, const RouteOpts& o) {
+    const c10::cuda::CUDAGuard guard(l.device());
+    const int n = as_int("route_experts", l.size(0)), E = (int)l.size(1);
+    Tensor inds = matrix(n, o.k, l, at::kInt), weights = matrix(n, o.k, l, at::kFloat), counts;
+    if (o.counts) counts = at::empty({E}, l.options().dtype(at::kInt));
+    check(p_rwkv_route_experts(l.const_data_ptr(), row_stride(l), bias ? bias->const_data_ptr<float>() : nullptr,
+                               inds.data_ptr<int>(), weights.data_ptr<float>(), o.counts ? counts.data_ptr<int>() : nullptr,
+                               n, E, o.k, o.groups, o.keep, o.top2, o.sigmoid, o.renorm, (float)o.scale, dtype_code(l),
+                               stream(l)),
+          "rwkv_route_experts", 1);
+    return {inds, weights, counts};
+}
+
+struct Route : torch::autograd::Function<Route> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& l, const std::optional<Tensor>& bias, const RouteOpts& o) {
+        auto [inds, weights, counts] = route_forward(l, bias, o);
+        ctx->save_for_backward({l, inds, weights});
+        ctx->saved_data["sigmoid"] = (int64_t)o.sigmoid;
+        ctx->saved_data["renorm"] = (int64_t)o.renorm;
+        ctx->saved_data["scale"] = o.scale;
+        ctx->set_materialize_grads(false);  // no zero tensors for the integer outputs
+        variable_list out{inds, weights}, whole{inds};
+        if (o.counts) out.push_back(counts), whole.push_back(counts);
+        ctx->mark_non_differentiable(whole);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        if (!grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &l = saved[0], &inds = saved[1], &weights = saved[2];
+        const c10::cuda::CUDAGuard guard(l.device());
+        const Tensor dw = grads[1].detach().to(at::kFloat).contiguous();
+        Tensor d = matrix(l.size(0), l.size(1), l, l.scalar_type());
+        const int code = l.scalar_type() == at::kFloat ? RWKV_F32 : l.scalar_type() == at::kHalf ? RWKV_F16 : RWKV_BF16;
+        check(p_rwkv_route_experts_backward(l.const_data_ptr(), row_stride(l), inds.const_data_ptr<int>(),
+                                            weights.const_data_ptr<float>(), dw.const_data_ptr<float>(), d.data_ptr(),
+                                            (int)l.size(0), (int)l.size(1), (int)inds.size(1),
+                                            (int)ctx->saved_data["sigmoid"].toInt(), (int)ctx->saved_data["renorm"].toInt(),
+                                            (float)ctx->saved_data["scale"].toDouble(), code, stream(l)),
+              "rwkv_route_experts_backward", 1);
+        return {once(d), Tensor(), Tensor()};
+    }
+};
+
+constexpr int64_t MAX_EXPERTS = 512, MAX_TOP_K = 32, MAX_GROUPS = 32;
+
+using Routed = std::variant<std::tuple<Tensor, Tensor>, std::tuple<Tensor, Tensor, Tensor>>;
+Routed route_experts(const Tensor& logits, int64_t top_k, const std::string& score, const std::optional<Tensor>& bias,
+                         int64_t n_groups, int64_t topk_groups, const std::string& group_score, bool renormalize,
+                         double scale, bool return_counts) {
+    if (score != "softmax" && score != "sigmoid") bad("route_experts: score must be 'softmax' or 'sigmoid', not '", score, "'");
+    if (group_score != "top2" && group_score != "max") bad("route_experts: group_score must be 'top2' or 'max', not '", group_score, "'");
+    if (logits.dim() < 1) bad("route_experts: logits must be (..., E)");
+    const int64_t E = logits.size(-1);
+    if (E < 1 || E > MAX_EXPERTS) bad("route_experts: 1 to ", MAX_EXPERTS, " experts, not ", E);
+    if (n_groups < 1 || n_groups > MAX_GROUPS || E % n_groups || topk_groups < 1 || topk_groups > n_groups)
+        bad("route_experts: ", n_groups, " groups of which ", topk_groups, " stay do not fit ", E, " experts (at most ",
+            MAX_GROUPS, " equal groups)");
+    const int64_t most = std::min(MAX_TOP_K, topk_groups * (E / n_groups));
+    if (top_k < 1 || top_k > most) bad("route_experts: top_k must be 1 to ", most, " here, not ", top_k);
+    std::optional<Tensor> b;
+    if (bias) {
+        if (bias->dim() != 1 || bias->size(0) != E || bias->device() != logits.device())
+            bad("route_experts: bias must be (E,) on the logits' device");
+        b = bias->detach().to(at::kFloat).contiguous();
+    }
+    dtype_code(logits);
+    on_gpu("route_experts", logits);
+    const Tensor l = rows_2d(logits);
+    const RouteOpts o{(int)top_k, score == "sigmoid", (int)n_groups, (int)topk_groups, group_score == "top2", renormalize, scale,
+                      return_counts};
+    Tensor inds, weights, counts;
+    if (wants_grad(logits)) {
+        const variable_list v = Route::apply(l, b, o);
+        inds = v[0], weights = v[1];
+        if (return_counts) counts = v[2];
+    } else {
+        std::tie(inds, weights, counts) = route_forward(l, b, o);
+    }
+    if (logits.dim() != 2) {
+        auto shape = logits.sizes().vec();
+        shape.back() = top_k;
+        inds = inds.view(shape), weights = weights.view(shape);
+    }
+    if (return_counts) return std::tuple{inds, weights, counts};
+    return std::tuple{inds, weights};
+}
+
+// ------------------------------------------------------------------ e4m3
+
+std::pair<Tensor, Tensor> quantize(const Tensor& x, int code) {
+    const int64_t M = x.size(0), K = x.size(1);
+    Tensor q = empty_e4m3(M, K, x), scale = empty_scale(M, K, x);
+    check(p_rwkv_quantize_fp8_rows(x.const_data_ptr(), row_stride(x), q.data_ptr(), q.stride(0), scale.data_ptr<float>(), (int)M,
+                                   (int)K, code, stream(x)),
+          "rwkv_quantize_fp8_rows", 1);
+    return {q, scale};
+}
+
+std::pair<Tensor, Tensor> quantize_fp8_rows(const Tensor& x) {
+    if (x.dim() != 2 || x.size(1) < 1) bad("quantize_fp8_rows: x must be (M, K) with K >= 1");
+    const int code = dtype_code(x);
+    on_gpu("quantize_fp8_rows", x);
+    const c10::cuda::CUDAGuard guard(x.device());
+    as_int("quantize_fp8_rows", x.size(0)), as_int("quantize_fp8_rows", x.size(1));
+    return quantize(rows_2d(x.detach()), code);
+}
+
+// x (M, K) times a weight whose checks have been made, the code that of x's type.
+Tensor linear(const Tensor& x, const Tensor& w, const Tensor& w_scale, int code) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int M = (int)x.size(0), K = (int)x.size(1), N = (int)w.size(0);
+    Tensor out = matrix(M, N, x, x.scalar_type()), ws;
+    const size_t nws = p_rwkv_fp8_linear_workspace_size(M, K);
+    if (nws) ws = at::empty({(int64_t)nws}, x.options().dtype(at::kByte));
+    check(p_rwkv_fp8_linear(x.const_data_ptr(), row_stride(x), w.const_data_ptr(), row_stride(w),
+                            w_scale.const_data_ptr<float>(), out.data_ptr(), N, nws ? ws.data_ptr() : nullptr, nws, M, N, K,
+                            code, stream(x)),
+          "rwkv_fp8_linear", nws ? 2 : 1);
+    return out;
+}
+
+struct Linear : torch::autograd::Function<Linear> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& w_scale, const Tensor& w_t,
+                          const Tensor& w_scale_t, int64_t code) {
+        ctx->save_for_backward({w_t, w_scale_t});
+        ctx->saved_data["code"] = code;
+        return linear(x, w, w_scale, (int)code);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        Tensor dx = linear(rows_2d(grads[0].detach()), saved[0], saved[1], (int)ctx->saved_data["code"].toInt());
+        return {once(dx), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor checked_scale(const char* name, const Tensor& w, const Tensor& scale, int64_t N, int64_t K, const Tensor& x) {
+    if (w.scalar_type() != at::kFloat8_e4m3fn || w.device() != x.device() || (K > 1 && w.stride(1) != 1) ||
+        scale.scalar_type() != at::kFloat || scale.device() != x.device() || scale.dim() != 2 || scale.size(0) != blocks(N) ||
+        scale.size(1) != blocks(K))
+        bad(name, ": the weight must be e4m3 (", N, ", ", K, ") with unit column stride and fp32 scales (", blocks(N), ", ",
+            blocks(K), ") on x's device");
+    return scale.contiguous();
+}
+
+Tensor fp8_linear(const Tensor& x, const Tensor& w, const Tensor& w_scale, const std::optional<Tensor>& w_t,
+                  const std::optional<Tensor>& w_scale_t) {
+    if (w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(1) || w.size(0) < 1 || w.size(1) < 1)
+        bad("fp8_linear: x ", x.sizes(), " and w ", w.sizes(), " do not fit (w is (N, K))");
+    const int code = dtype_code(x);
+    on_gpu("fp8_linear", x);
+    const int64_t N = w.size(0), K = w.size(1);
+    const Tensor s = checked_scale("fp8_linear", w, w_scale, N, K, x), x2 = rows_2d(x);
+    as_int("fp8_linear", x2.size(0));
+    Tensor y;
+    if (wants_grad(x)) {
+        if (!w_t || !w_scale_t) {
+            throw std::runtime_error("fp8_linear: an input that requires grad needs the transposed weight "
+                                     "(transpose_fp8_weight) for the gradient");
+        }
+        if (w_t->dim() != 2 || w_t->size(0) != K || w_t->size(1) != N) bad("fp8_linear: w_t must be (K, N)");
+        y = Linear::apply(x2, w, s, *w_t, checked_scale("fp8_linear", *w_t, *w_scale_t, K, N, x), (int64_t)code);
+    } else {
+        y = linear(x2, w, s, code);
+    }
+    if (x.dim() == 2) return y;
+    auto shape = x.sizes().vec();
+    shape.back() = N;
+    return y.view(shape);
+}
+
+// An expert weight (E, N, K) with its scales (E, ceil(N / 128), ceil(K / 128)).
+struct Weight {
+    Tensor q, scale;
+    int64_t pitch() const { return q.size(1) > 1 ? q.stride(1) : pitch16(q.size(2)); }
+};
+Weight checked_weight(const Tensor& q, const Tensor& scale, int64_t E, int64_t N, int64_t K, const Tensor& x) {
+    if (q.dim() != 3 || q.scalar_type() != at::kFloat8_e4m3fn || q.device() != x.device() || q.size(0) != E || q.size(1) != N ||
+        q.size(2) != K || q.numel() == 0)
+        bad("fp8_experts: a weight must be e4m3 (", E, ", ", N, ", ", K, ") on the rows' device");
+    if (scale.dim() != 3 || scale.scalar_type() != at::kFloat || scale.device() != x.device() || scale.size(0) != E ||
+        scale.size(1) != blocks(N) || scale.size(2) != blocks(K))
+        bad("fp8_experts: a weight's scales must be fp32 (E, ceil(N / 128), ceil(K / 128)) on the rows' device");
+    const Weight w{q, scale.contiguous()};
+    if ((K > 1 && q.stride(2) != 1) || w.pitch() % 16 || w.pitch() < K || (E > 1 && q.stride(0) % 16) ||
+        reinterpret_cast<uintptr_t>(q.const_data_ptr()) % 16)
+        bad("fp8_experts: a weight's rows must be 16-byte aligned with unit column stride (quantize_fp8_weight lays them out so)");
+    return w;
+}
+
+Tensor experts(const Tensor& x, const Weight& key, const Weight& val, const Tensor& offsets, int code) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int M = (int)x.size(0), C = (int)x.size(1), E = (int)key.q.size(0), D = (int)key.q.size(1);
+    Tensor out = matrix(M, C, x, x.scalar_type());
+    const size_t nws = p_rwkv_fp8_experts_workspace_size(M, C, D, E);
+    const Tensor ws = at::empty({(int64_t)nws}, x.options().dtype(at::kByte));
+    check(p_rwkv_fp8_experts(x.const_data_ptr(), row_stride(x), key.q.const_data_ptr(), key.pitch(), key.q.stride(0),
+                             key.scale.const_data_ptr<float>(), val.q.const_data_ptr(), val.pitch(), val.q.stride(0),
+                             val.scale.const_data_ptr<float>(), offsets.const_data_ptr<int>(), out.data_ptr(), C,
+                             ws.data_ptr(), nws, M, C, D, E, code, stream(x)),
+          "rwkv_fp8_experts", 3);
+    return out;
+}
+
+// rows (M, K) quantised times w, grouped, in x's type (a step of the backward pass).
+Tensor product(const std::pair<Tensor, Tensor>& a, const Weight& w, const Tensor& offsets, const Tensor& x, int code) {
+    const int64_t M = a.first.size(0), K = a.first.size(1), N = w.q.size(1), E = w.q.size(0);
+    Tensor out = matrix(M, N, x, x.scalar_type());
+    check(p_rwkv_fp8_gemm(a.first.const_data_ptr(), row_stride(a.first), a.second.const_data_ptr<float>(),
+                          w.q.const_data_ptr(), w.pitch(), w.q.stride(0), w.scale.const_data_ptr<float>(),
+                          offsets.const_data_ptr<int>(), out.data_ptr(), N, nullptr, (int)M, (int)N, (int)K, (int)E, 0, code,
+                          stream(x)),
+          "rwkv_fp8_gemm", 1);
+    return out;
+}
+
+struct Experts : torch::autograd::Function<Experts> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& key, const Tensor& key_scale, const Tensor& val,
+                          const Tensor& val_scale, const Tensor& offsets, const Tensor& key_t, const Tensor& key_t_scale,
+                          const Tensor& val_t, const Tensor& val_t_scale, int64_t code) {
+        ctx->save_for_backward({x, offsets, key, key_scale, key_t, key_t_scale, val_t, val_t_scale});
+        ctx->saved_data["code"] = code;
+        return experts(x, {key, key_scale}, {val, val_scale}, offsets, (int)code);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto s = ctx->get_saved_variables();
+        const Tensor x = s[0].detach(), &offsets = s[1], dy = rows_2d(grads[0].detach());
+        const int code = (int)ctx->saved_data["code"].toInt();
+        const c10::cuda::CUDAGuard guard(x.device());
+        // u again rather than kept from the forward pass (there it never leaves the key product's kernel)
+        const Tensor u = product(quantize(x, code), {s[2], s[3]}, offsets, x, code);
+        const Tensor dh = product(quantize(dy, code), {s[6], s[7]}, offsets, x, code);
+        const int64_t M = u.size(0), D = u.size(1);
+        Tensor q = empty_e4m3(M, D, x), scale = empty_scale(M, D, x);
+        check(p_rwkv_quantize_fp8_relu_sq_grad(dh.const_data_ptr(), u.const_data_ptr(), D, q.data_ptr(), q.stride(0),
+                                               scale.data_ptr<float>(), (int)M, (int)D, code, stream(x)),
+              "rwkv_quantize_fp8_relu_sq_grad", 1);
+        variable_list out(11);
+        out[0] = once(product({q, scale}, {s[4], s[5]}, offsets, x, code));
+        return out;
+    }
+};
+
+Tensor fp8_experts(const Tensor& rows, const Tensor& key, const Tensor& key_scale, const Tensor& value,
+                   const Tensor& value_scale, const Tensor& offsets, const std::optional<std::vector<Tensor>>& transposed) {
+    if (rows.dim() != 2 || key.dim() != 3 || key.size(2) != rows.size(1))
+        bad("fp8_experts: rows ", rows.sizes(), " and key ", key.sizes(), " do not fit (key (E, D, C), value (E, C, D))");
+    const int code = dtype_code(rows);
+    on_gpu("fp8_experts", rows);
+    const int64_t E = key.size(0), D = key.size(1), C = key.size(2);
+    const Weight k = checked_weight(key, key_scale, E, D, C, rows), v = checked_weight(value, value_scale, E, C, D, rows);
+    if (offsets.scalar_type() != at::kInt || offsets.numel() != E + 1 || !offsets.is_contiguous() ||
+        offsets.device() != rows.device())
+        bad("fp8_experts: offsets must be a contiguous int32 (E + 1,) tensor on the rows' device");
+    const Tensor x = rows_2d(rows);
+    as_int("fp8_experts", x.size(0));
+    if (!wants_grad(rows)) return experts(x, k, v, offsets, code);
+    if (!transposed || transposed->size() != 4) {
+        throw std::runtime_error("fp8_experts: rows that require grad need the transposed weights for the gradient");
+    }
+    const auto& t = *transposed;
+    const Weight kt = checked_weight(t[0], t[1], E, C, D, rows), vt = checked_weight(t[2], t[3], E, D, C, rows);
+    return Experts::apply(x, k.q, k.scale, v.q, v.scale, offsets, kt.q, kt.scale, vt.q, vt.scale, (int64_t)code);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_rwkv_host, m) {
+    m.def("bind", &bind);
+    m.def("launches", [] { return g_launches.load(); });
+    // A launch may wait for room in the stream: other threads run meanwhile.
+    const py::call_guard<py::gil_scoped_release> unlocked;
+    m.def("route_experts", &route_experts, unlocked);
+    m.def("quantize_fp8_rows", &quantize_fp8_rows, unlocked);
+    m.def("fp8_linear", &fp8_linear, unlocked);
+    m.def("fp8_experts", &fp8_experts, unlocked);
+}

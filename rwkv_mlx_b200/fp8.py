@@ -2,7 +2,8 @@
 
 Activations carry one scale for each 128 values of a row, weights one for each 128 x 128 block
 (``csrc/fp8_quant.cu``); products accumulate in fp32 and apply the scales block by block
-(``csrc/fp8_gemm.cu``, ``csrc/fp8_gemm_tc.cu``).  The reference has no 8-bit path; these are the
+(``csrc/fp8_gemm.cu``, ``csrc/fp8_gemm_tc.cu``).  The calls of a few microseconds and the gradients are
+made in C++ (``csrc/host/expert_ops.cpp``).  The reference has no 8-bit path; these are the
 weights-in-8-bits forms of the projections of rwkv_mlx/model.py:245-263 and of the experts of
 rwkv_mlx/moe.py:231-239.
 
@@ -39,20 +40,7 @@ def quantize_fp8_rows(x: torch.Tensor):
 
     For each block of 128 values of a row, a = max|x| (at least 1e-30): scale = a / 448,
     q = e4m3(x * (448 / a)).  A NaN stays NaN in its place; an infinity makes its block NaN."""
-    if x.dim() != 2 or x.shape[1] < 1:
-        raise ValueError("quantize_fp8_rows: x must be (M, K) with K >= 1")
-    code = nat.dtype_code(x)
-    x = nat.rows_2d(x)
-    M, K = x.shape
-    dev = x.device
-    q = _empty_e4m3(M, K, dev)
-    scale = _empty_scale(M, K, dev)
-    L = nat.lib()
-    with nat.on_device(dev):
-        rc = L.rwkv_quantize_fp8_rows(x.data_ptr(), nat.row_stride(x), q.data_ptr(), q.stride(0), scale.data_ptr(), M, K,
-                                      code, nat.stream_ptr(dev))
-    nat.check(rc, "rwkv_quantize_fp8_rows")
-    return q, scale
+    return nat.host().quantize_fp8_rows(x)
 
 
 def quantize_fp8_weight(w: torch.Tensor):
@@ -168,40 +156,6 @@ def fp8_matmul_relu_sq_quantized(a: torch.Tensor, a_scale: torch.Tensor, w: torc
     return q, scale
 
 
-def _linear(x2d, w, w_scale):
-    """x2d has unit column stride; the weight is checked here, the rest by the library."""
-    M, K = x2d.shape
-    dev = x2d.device
-    if w.dtype != E4M3 or w.device != dev or w_scale.dtype != torch.float32 or w_scale.device != dev \
-            or w_scale.shape != (_blocks(w.shape[0]), _blocks(K)) or (K > 1 and w.stride(1) != 1):
-        raise ValueError(f"fp8_linear: the weight must be e4m3 (N, {K}) with unit column stride and fp32 scales "
-                         "(ceil(N / 128), ceil(K / 128)) on x's device")
-    N = w.shape[0]
-    code = nat.dtype_code(x2d)
-    out = torch.empty_strided((M, N), (N, 1), dtype=x2d.dtype, device=dev)
-    L = nat.lib()
-    nws = L.rwkv_fp8_linear_workspace_size(M, K)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-    with nat.on_device(dev):
-        rc = L.rwkv_fp8_linear(x2d.data_ptr(), nat.row_stride(x2d), w.data_ptr(), nat.row_stride(w),
-                               w_scale.contiguous().data_ptr(), out.data_ptr(), N, nat.ptr(ws), nws, M, N, K, code,
-                               nat.stream_ptr(dev))
-    nat.check(rc, "rwkv_fp8_linear")
-    return out
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x2d, w, w_scale, w_t, w_scale_t):
-        ctx.save_for_backward(w_t, w_scale_t)
-        return _linear(x2d, w, w_scale)
-
-    @staticmethod
-    @nat.first_order
-    def backward(ctx, dy):
-        return _linear(nat.rows_2d(dy), *ctx.saved_tensors), None, None, None, None
-
-
 def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, w_t: torch.Tensor | None = None,
                w_scale_t: torch.Tensor | None = None) -> torch.Tensor:
     """x (..., K) @ w^T -> (..., N) in x's dtype: x is quantised in the call, w (N, K) is held in e4m3.
@@ -209,56 +163,7 @@ def fp8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, w_t: tor
     The weight is frozen.  For an x that requires grad, pass the transposed layout
     (:func:`transpose_fp8_weight`, kept beside the weight): dx = q(dy) @ w runs on the same kernels,
     with dy quantised like x."""
-    if w.dim() != 2 or x.shape[-1] != w.shape[1]:
-        raise ValueError(f"fp8_linear: x {tuple(x.shape)} and w {tuple(w.shape)} do not fit (w is (N, K))")
-    x2 = nat.rows_2d(x)
-    if x.requires_grad and torch.is_grad_enabled():
-        if w_t is None or w_scale_t is None:
-            raise RuntimeError("fp8_linear: an input that requires grad needs the transposed weight "
-                               "(transpose_fp8_weight) for the gradient")
-        if w_t.shape != (w.shape[1], w.shape[0]):
-            raise ValueError("fp8_linear: w_t must be (K, N)")
-        y = _Linear.apply(x2, w, w_scale, w_t, w_scale_t)
-    else:
-        y = _linear(x2, w, w_scale)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
-
-
-def _experts(x, key, key_scale, value, value_scale, offsets, C, D, E, ldk, ldv):
-    M, dev = x.shape[0], x.device
-    out = torch.empty_strided((M, C), (C, 1), dtype=x.dtype, device=dev)
-    L = nat.lib()
-    nws = L.rwkv_fp8_experts_workspace_size(M, C, D, E)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
-    with nat.on_device(dev):
-        rc = L.rwkv_fp8_experts(x.data_ptr(), nat.row_stride(x), key.data_ptr(), ldk, key.stride(0), key_scale.data_ptr(),
-                                value.data_ptr(), ldv, value.stride(0), value_scale.data_ptr(), nat.ptr(offsets),
-                                out.data_ptr(), C, ws.data_ptr(), nws, M, C, D, E, nat.dtype_code(x), nat.stream_ptr(dev))
-    nat.check(rc, "rwkv_fp8_experts")
-    return out
-
-
-class _Experts(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weights, transposed, offsets, dims):
-        ctx.save_for_backward(x, offsets, *weights[:2], *transposed)
-        return _experts(x, *weights, offsets, *dims)
-
-    @staticmethod
-    @nat.first_order
-    def backward(ctx, dy):
-        x, offsets, key, key_scale, key_t, key_t_scale, value_t, value_t_scale = ctx.saved_tensors
-        # u again rather than kept from the forward pass (there it never leaves the key product's kernel)
-        u = fp8_matmul(*quantize_fp8_rows(x), key, key_scale, offsets, out_dtype=x.dtype)
-        dh = fp8_matmul(*quantize_fp8_rows(dy), value_t, value_t_scale, offsets, out_dtype=x.dtype)
-        M, D = u.shape
-        q, scale = _empty_e4m3(M, D, x.device), _empty_scale(M, D, x.device)
-        L = nat.lib()
-        with nat.on_device(x.device):
-            rc = L.rwkv_quantize_fp8_relu_sq_grad(dh.data_ptr(), u.data_ptr(), D, q.data_ptr(), q.stride(0),
-                                                  scale.data_ptr(), M, D, nat.dtype_code(u), nat.stream_ptr(x.device))
-        nat.check(rc, "rwkv_quantize_fp8_relu_sq_grad")
-        return fp8_matmul(q, scale, key_t, key_t_scale, offsets, out_dtype=x.dtype), None, None, None, None
+    return nat.host().fp8_linear(x, w, w_scale, w_t, w_scale_t)
 
 
 def fp8_experts(rows: torch.Tensor, key: torch.Tensor, key_scale: torch.Tensor, value: torch.Tensor,
@@ -271,21 +176,4 @@ def fp8_experts(rows: torch.Tensor, key: torch.Tensor, key_scale: torch.Tensor, 
     The weights are frozen.  For rows that require grad, pass ``transposed`` = (key_t, key_t_scale,
     value_t, value_t_scale), the two weights through :func:`transpose_fp8_weight`: with u = q(x) key^T,
     dx = q(q(dy) value * 2 relu(u)) key, the quantisations' own derivatives taken as 1."""
-    if rows.dim() != 2 or key.dim() != 3 or value.dim() != 3 or value.shape != (key.shape[0], key.shape[2], key.shape[1]) \
-            or key.shape[2] != rows.shape[1]:
-        raise ValueError(f"fp8_experts: rows {tuple(rows.shape)}, key {tuple(key.shape)} and value {tuple(value.shape)} "
-                         "do not fit (key (E, D, C), value (E, C, D))")
-    nat.dtype_code(rows)
-    x = nat.rows_2d(rows)
-    C, dev = x.shape[1], x.device
-    key, key_scale, E, D, ldk = _check_weight("fp8_experts", key, key_scale, C, dev)
-    value, value_scale, _, _, ldv = _check_weight("fp8_experts", value, value_scale, D, dev)
-    _check_offsets("fp8_experts", offsets, E, dev)
-    if rows.requires_grad and torch.is_grad_enabled():
-        if transposed is None:
-            raise RuntimeError("fp8_experts: rows that require grad need the transposed weights for the gradient")
-        key_t, value_t = transposed[0], transposed[2]
-        if key_t.shape != (E, C, D) or value_t.shape != (E, D, C):
-            raise ValueError("fp8_experts: transposed must be key (E, C, D) and value (E, D, C) with their scales")
-        return _Experts.apply(x, (key, key_scale, value, value_scale), transposed, offsets, (C, D, E, ldk, ldv))
-    return _experts(x, key, key_scale, value, value_scale, offsets, C, D, E, ldk, ldv)
+    return nat.host().fp8_experts(rows, key, key_scale, value, value_scale, offsets, transposed)
